@@ -483,6 +483,133 @@ int vk_tree_verify_plan(const vk_pool* pool, const vk_tree_args* a, vk_tree_plan
  * position so sibling branches do not collide, and a node sees itself. */
 int vk_tree_verify(vk_ctx* ctx, vk_pool* pool, const vk_tree_args* a, void* stream);
 
+/* ---- sparse decode -----------------------------------------------------------
+ * Attention of a decode step over a few pages of a long context, chosen for each
+ * query by a cheap score. No counterpart in the reference, whose kernels read the
+ * whole context (kernels.metal:440-501). A key index holds, for every layer, page
+ * and KV head, the lower and upper bound of the page's keys in each dim, as int8
+ * codes with one fp32 scale: 2 * head_dim + 4 bytes (head_dim rounded up to 64 or
+ * 128) beside a page's block_size * head_dim elements of K. A decode step appends
+ * its tokens (vk_append_rope), brings the index up to date (vk_index_update), and
+ * chooses and attends (vk_select_decode). */
+typedef struct vk_key_index vk_key_index;
+
+/* An index of all layers of the pool, zero-filled (destroy it before the pool). */
+int vk_index_create(vk_ctx* ctx, vk_pool* pool, vk_key_index** out);
+int vk_index_destroy(vk_key_index* index);
+/* HBM held by the index. */
+int vk_index_bytes(const vk_key_index* index, uint64_t* out);
+
+/* Compute one layer's bounds of every page that holds a position in
+ * [first_tokens[s], context_lens[s]) of sequence s, from the keys as the pool stores
+ * them (code * scale for the I8 types) at the page's positions below
+ * context_lens[s]. Call it when those positions have changed: after an append, a
+ * tree commit, a page copy or a NIXL unpack. first_tokens NULL = 0. max_tokens is a
+ * host upper bound of context_lens[s] - first_tokens[s] (0 = max_context_len); pages
+ * past it are not brought up to date. For each dim lo = min, hi = max of the keys;
+ * with top = max |lo|, |hi| over the dims, scale = top / 127, inv = 127 / top (0
+ * where that is not finite) in fp32, codes rint(lo * inv) and rint(hi * inv). A page
+ * with a key that is not finite has the scale +infinity. All pointers are device
+ * pointers; tables, rows and lengths as in vk_decode_args. A page id outside the
+ * pool is skipped and reported (VK_MISUSE_PAGE_OUT_OF_POOL). Of a page that several
+ * sequences of the call share, all must hold the same number of tokens. */
+int vk_index_update(vk_ctx* ctx, vk_key_index* index, int32_t layer, const int32_t* block_tables,
+                    int32_t bt_stride, const int32_t* seq_rows, const int32_t* first_tokens,
+                    const int32_t* context_lens, int32_t n_seqs, int32_t max_context_len,
+                    int32_t max_tokens, void* stream);
+
+/* Read one layer's bounds of listed pages (dev int32 [n_pages] page ids) as values:
+ * lower and upper, dev fp32 [n_pages][n_kv_heads][head_dim], 16-byte aligned
+ * (code * scale; -infinity and +infinity for a page whose scale is infinite). A page
+ * id outside the pool reads zeros and is reported. */
+int vk_index_read(vk_ctx* ctx, vk_key_index* index, int32_t layer, const int32_t* pages,
+                  int32_t n_pages, float* lower, float* upper, void* stream);
+
+typedef struct vk_sparse_args {
+  int32_t layer;
+  const void* q;              /* dev [S][n_heads][head_dim] of q_dtype         */
+  int32_t q_dtype;            /* VK_DT_*                                       */
+  float* out;                 /* dev fp32 [S][n_heads][head_dim] (attention)   */
+  int32_t* pages;             /* dev [S][n_kv_heads][n_pages]: places in the sequence's
+                                 table row (0 = its first page); written by the selection,
+                                 read by the attention                          */
+  int32_t n_pages;            /* length of a list                              */
+  int32_t n_first;            /* selection: the first n_first and the last n_last pages of a */
+  int32_t n_last;             /* context are always listed; n_first + n_last <= n_pages */
+  const int32_t* block_tables;/* dev [rows][bt_stride]; NULL = the pool's slot table */
+  int32_t bt_stride;          /* ignored when block_tables is NULL             */
+  const int32_t* seq_rows;    /* dev [S] row of each sequence; NULL = 0..S-1   */
+  const int32_t* context_lens;/* dev [S] tokens to attend (incl. the new one)  */
+  int32_t n_seqs;             /* S; a table row may occur in several, with its own
+                                 context_len each (the queries of a draft or a prompt) */
+  int32_t n_heads;            /* query heads H: n_kv_heads times a group of up to 32 */
+  int32_t max_context_len;    /* host upper bound of context_lens              */
+  float scale;                /* softmax scale; 0 = 1/sqrt(head_dim)           */
+  void* workspace;            /* dev scratch; NULL = owned by ctx (calls on one ctx that
+                                 overlap in time, and graphs that may, then pass their own).
+                                 Needs no initialisation. A call under stream capture does
+                                 not grow the context's. */
+  uint64_t workspace_bytes;
+} vk_sparse_args;
+
+/* Bytes of workspace that any of the three calls below needs for these arguments. */
+int vk_sparse_workspace(const vk_pool* pool, const vk_sparse_args* a, uint64_t* bytes);
+
+/* Choose n_pages pages of each (sequence, KV head): the first n_first, the last
+ * n_last, and of the others those of the highest score, ties to the lower page. The
+ * score of page p is the largest over the group's heads h of
+ *     fp32(fp32(dot * scale_p) * scale_h),
+ *     dot = sum over d of (c_d < 0 ? c_d * lo_d : c_d * hi_d),
+ * an estimate of the largest q . k in the page: lo, hi the page's codes, c the codes
+ * of q, c_d = rint(q_d * inv), scale_h = top / 127, inv = 127 / top (0 where that is
+ * not finite), top = max |q_d|. dot is a whole number, so the choice does not depend
+ * on how it is computed. A page of infinite scale scores +infinity; the scores of a
+ * query that is not finite are 0. Lists are in ascending order; a context of fewer pages
+ * lists them all and ends in -1. Writes a->pages; a->out and a->scale are not used. */
+int vk_select_pages(vk_ctx* ctx, vk_key_index* index, const vk_sparse_args* a, void* stream);
+
+/* Decode attention over the listed pages: softmax(scale * q . k) v over the tokens
+ * below context_lens[s] of the pages that list [s][KV head] names. Entries below 0 or
+ * past the context name nothing; a page listed twice counts twice; rows with no
+ * token are 0. a->n_first and a->n_last are checked, not used. Results are those of
+ * fp32 arithmetic over the stored values to about 2^-20 of the largest, whatever the
+ * types. */
+int vk_sparse_decode(vk_ctx* ctx, vk_pool* pool, const vk_sparse_args* a, void* stream);
+
+/* vk_select_pages, then vk_sparse_decode over its lists, on one stream. */
+int vk_select_decode(vk_ctx* ctx, vk_key_index* index, const vk_sparse_args* a, void* stream);
+
+/* ---- log probabilities ---------------------------------------------------------
+ * The step from logits to tokens: what a served answer reports of its tokens, and
+ * the target model's token after every node of a draft tree (TreeVerifyResult,
+ * speculative.rs:36-40, from which vk_tree_commit's paths follow). */
+typedef struct vk_logprob_args {
+  const void* logits;         /* dev [n_rows][row_stride], vocab of each row read */
+  int32_t dtype;              /* VK_DT_* of the logits                          */
+  int64_t row_stride;         /* elements from a row to the next; 0 = vocab     */
+  int32_t n_rows;
+  int32_t vocab;              /* up to 2^28                                     */
+  float scale;                /* x = scale * logit (1 / temperature); 0 = 1     */
+  const int32_t* tokens;      /* dev [n_rows][n_tokens] given tokens            */
+  int32_t n_tokens;           /* 0 = none                                       */
+  float* token_logprobs;      /* dev [n_rows][n_tokens]                         */
+  float* entropy;             /* dev [n_rows]; NULL = not computed              */
+  int32_t* top_ids;           /* dev [n_rows][n_top], the most probable first,  */
+  float* top_logprobs;        /* ties to the lower id                           */
+  int32_t n_top;              /* 0..32, at most vocab                           */
+  void* workspace;            /* as in vk_sparse_args                           */
+  uint64_t workspace_bytes;
+} vk_logprob_args;
+
+/* log p(t) = x_t - log sum_v e^(x_v), entropy -sum p log p (natural logarithms), sums
+ * in fp32. A logit of -infinity has probability 0; a row of nothing else has log
+ * probabilities of -infinity, the entropy 0 and the lowest ids on top. A row with NaN
+ * or +infinity has NaN log probabilities and entropy (NaN counts as -infinity in the
+ * choice of top_ids). A given token outside the vocabulary has -infinity. Reads the
+ * logits once. */
+int vk_token_logprobs(vk_ctx* ctx, const vk_logprob_args* a, void* stream);
+int vk_token_logprobs_workspace(const vk_ctx* ctx, const vk_logprob_args* a, uint64_t* bytes);
+
 /* Ancestor mask of a draft tree given as parent indices (parents[0] = -1 for
  * the root, parents[i] < i otherwise): mask_out[i] has bit j set when node j is
  * node i or one of its ancestors. Host only.

@@ -1,7 +1,9 @@
 """Build the gfx950 code object and the C-ABI host library in-tree.
 
-  velokv/velokv_gfx950.co  hipcc --offload-arch=gfx950 --offload-device-only (raw code object)
-  velokv/libvelokv.so      g++ over the HIP runtime API (host code only)
+  velokv/velokv_gfx950.co         hipcc --offload-arch=gfx950 --offload-device-only (raw code objects)
+  velokv/velokv_sparse_gfx950.co
+  velokv/velokv_logits_gfx950.co
+  velokv/libvelokv.so             g++ over the HIP runtime API (host code only)
 
 Run `python velo-core_amd/build.py` or __graft_entry__.build().
 """
@@ -10,6 +12,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -34,11 +37,16 @@ def _run(cmd):
     return r.stdout
 
 
-def build_code_object():
-    out = os.path.join(PKG, "velokv_gfx950.co")
+# source -> code object
+CODE_OBJECTS = {"velokv_kernels.hip": "velokv_gfx950.co", "velokv_sparse.hip": "velokv_sparse_gfx950.co",
+                "velokv_logits.hip": "velokv_logits_gfx950.co"}
+
+
+def build_code_object(source="velokv_kernels.hip"):
+    out = os.path.join(PKG, CODE_OBJECTS[source])
     tmp = out + ".tmp"
     _run([os.path.join(ROCM, "bin", "hipcc"), *HIPCC_FLAGS, f"-I{CSRC}", f"-I{INCLUDE}",
-          os.path.join(CSRC, "velokv_kernels.hip"), "-o", tmp])
+          os.path.join(CSRC, source), "-o", tmp])
     os.replace(tmp, out)
     return out
 
@@ -67,16 +75,17 @@ def build_host_library(sanitize: bool = False):
     _run(["g++", "-O1" if sanitize else "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wextra",
           "-Wno-unused-parameter", *san,
           "-D__HIP_PLATFORM_AMD__", f"-I{ROCM}/include", f"-I{INCLUDE}", f"-I{CSRC}",
-          os.path.join(CSRC, "velokv_host.cpp"), os.path.join(CSRC, "velokv_radix.cpp"), noalloc, "-o", tmp,
+          *(os.path.join(CSRC, f"velokv_{name}.cpp") for name in ("host", "radix", "sparse", "logits")), noalloc, "-o", tmp,
           f"-L{ROCM}/lib", "-lamdhip64", f"-Wl,-rpath,{ROCM}/lib", "-ldl"])
     os.replace(tmp, out)
     return out
 
 
 def build():
-    co = build_code_object()
-    so = build_host_library()
-    return co, so
+    with ThreadPoolExecutor(len(CODE_OBJECTS)) as pool:
+        objects = pool.map(build_code_object, CODE_OBJECTS)
+        so = build_host_library()
+        return *objects, so
 
 
 def sanitizer_runtime():

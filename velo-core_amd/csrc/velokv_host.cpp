@@ -22,8 +22,7 @@
 #include <unordered_map>
 #include <vector>
 
-#include "velokv_params.h"
-#include "velokv_plan.h"
+#include "velokv_internal.h"
 
 using namespace velokv;
 
@@ -31,28 +30,9 @@ namespace {
 
 thread_local std::string g_last_error;
 
-int fail(int code, const char* fmt, ...) {
-  char buf[1024];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof buf, fmt, ap);
-  va_end(ap);
-  g_last_error = buf;
-  return code;
-}
-
-#define HIP_TRY(expr)                                                              \
-  do {                                                                             \
-    hipError_t _e = (expr);                                                        \
-    if (_e != hipSuccess)                                                          \
-      return fail(VK_ERR_HIP, "%s failed: %s", #expr, hipGetErrorString(_e));     \
-  } while (0)
-
 constexpr int kMaxPageTiles = 16;  // pages of 16 * k tokens, k <= 16 (up to 256 tokens)
 constexpr int kHD = 128;  // head_dim the kernels are built for
 constexpr int kMaxTreeNodes = 32;     // one 32-bit mask row per node
-
-uint64_t align_up(uint64_t x, uint64_t a) { return (x + a - 1) / a * a; }
 
 int kv_stile(int kv, int bs) {
   if (kv == VK_KV_I8_BLK) return 2;
@@ -80,17 +60,28 @@ std::string append_kernel_name(int kv_type, int head_dim) {
   return "vk_append_kv" + std::to_string(kv_type) + (kv_type == VK_KV_I8_BLK && tile_hd(head_dim) != kHD ? "_d64" : "");
 }
 
-std::string default_code_object_path() {
+// Path of a file next to this library.
+std::string beside_library(const char* file) {
   Dl_info info;
   if (dladdr(reinterpret_cast<void*>(&vk_ctx_create), &info) && info.dli_fname) {
     std::string p(info.dli_fname);
     const size_t slash = p.find_last_of('/');
-    return (slash == std::string::npos ? std::string(".") : p.substr(0, slash)) + "/velokv_gfx950.co";
+    return (slash == std::string::npos ? std::string(".") : p.substr(0, slash)) + "/" + file;
   }
-  return "velokv_gfx950.co";
+  return file;
 }
 
 }  // namespace
+
+int velokv::fail(int code, const char* fmt, ...) {
+  char buf[1024];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  g_last_error = buf;
+  return code;
+}
 
 // Error channel shared with the other translation units of the library
 // (velokv_radix.cpp, velokv_noalloc.hip): sets the calling thread's
@@ -103,55 +94,6 @@ int vk_internal_set_error(int code, const char* msg) {
 // Resolves the no-alloc scratch of `device` (velokv_noalloc.hip); the device
 // must be current.
 int vk_internal_noalloc_init(int device);
-
-struct vk_ctx {
-  int device = 0;
-  std::string arch;
-  hipModule_t module = nullptr;
-  std::unordered_map<std::string, hipFunction_t> fns;
-  // threads per workgroup each kernel was compiled for (__launch_bounds__), read
-  // once at vk_ctx_create: a launch with more faults the device, so launch()
-  // refuses it
-  std::unordered_map<std::string, int> max_threads;
-  std::mutex ws_mu;
-  void* ws = nullptr;
-  uint64_t ws_bytes = 0;
-  // Buffers the context's workspace outgrew: a call on another host thread may
-  // still have kernels queued that use one, so they are freed only by
-  // vk_ctx_destroy (growth is rare: once per new largest shape).
-  std::vector<void*> ws_retired;
-  uint32_t* err_word = nullptr;  // device: misuse flags (VK_MISUSE_*) or-ed by the kernels
-  int decode_kind = VK_DECODE_AUTO;
-  int decode_sched = VK_SCHED_AUTO;
-  int n_cu = 256;
-  std::mutex res_mu;                                   // guards resident, wg_resident
-  std::unordered_map<std::string, int64_t> resident;  // kernel -> resident waves
-  std::unordered_map<std::string, WgResident> wg_resident;
-
-  hipFunction_t fn(const std::string& name) const {
-    auto it = fns.find(name);
-    return it == fns.end() ? nullptr : it->second;
-  }
-};
-
-struct vk_pool {
-  vk_ctx* ctx = nullptr;
-  vk_pool_desc desc{};
-  PoolGeom geom{};
-  uint8_t* base = nullptr;
-  uint64_t bytes = 0;
-  int32_t* table = nullptr;  // [max_slots][max_pages_per_slot]
-  uint64_t table_bytes = 0;
-  // I8_BLK: per block, (epoch << 32 | first token) of the last append run on it,
-  // so that a call with two runs on one block is reported (VK_MISUSE_BLK_SPLIT_RUN)
-  unsigned long long* claim = nullptr;
-  std::atomic<uint32_t> epoch{0};
-  uint32_t next_epoch() {
-    uint32_t e = ++epoch;
-    while (e == 0) e = ++epoch;  // 0 marks a never-claimed block
-    return e;
-  }
-};
 
 namespace {
 
@@ -207,34 +149,6 @@ std::string tree_name(int kv, int g, int rt, int qt, bool d64 = false) {
          "_q" + std::to_string(qt);
 }
 
-int set_device(const vk_ctx* ctx) {
-  HIP_TRY(hipSetDevice(ctx->device));
-  return VK_OK;
-}
-
-// A workgroup shape the kernel was compiled for: at least one thread and at most
-// its __launch_bounds__ (HIP_FUNC_ATTRIBUTE_MAX_THREADS_PER_BLOCK).
-int check_launch_shape(const vk_ctx* ctx, const char* name, uint64_t threads) {
-  auto it = ctx->max_threads.find(name);
-  if (it == ctx->max_threads.end()) return fail(VK_ERR_NOT_WIRED, "kernel %s is not in the code object", name);
-  if (threads == 0 || threads > (uint64_t)it->second)
-    return fail(VK_ERR_BAD_ARG, "kernel %s launched with %llu threads per workgroup; it was compiled for at most %d",
-                name, (unsigned long long)threads, it->second);
-  return VK_OK;
-}
-
-template <typename P>
-int launch(const vk_ctx* ctx, const char* name, dim3 grid, dim3 block, const P& params, void* stream) {
-  hipFunction_t f = ctx->fn(name);
-  if (!f) return fail(VK_ERR_NOT_WIRED, "kernel %s is not in the code object", name);
-  int rc = check_launch_shape(ctx, name, (uint64_t)block.x * block.y * block.z);
-  if (rc) return rc;
-  void* args[] = {const_cast<P*>(&params)};
-  HIP_TRY(hipModuleLaunchKernel(f, grid.x, grid.y, grid.z, block.x, block.y, block.z, 0,
-                                reinterpret_cast<hipStream_t>(stream), args, nullptr));
-  return VK_OK;
-}
-
 // Waves of a kernel that fit on the device at once, launched with workgroups of
 // `block` threads (one wave each by default).
 int64_t resident_waves(vk_ctx* ctx, const std::string& name, int block = 64) {
@@ -265,11 +179,35 @@ WgResident wg_resident_waves(vk_ctx* ctx, const std::string& name) {
   return r;
 }
 
-int check_pool(const vk_ctx* ctx, const vk_pool* pool) {
-  if (!ctx) return fail(VK_ERR_NOT_WIRED, "context is null");
-  if (!pool) return fail(VK_ERR_NOT_WIRED, "pool is null");
-  if (pool->ctx != ctx) return fail(VK_ERR_BAD_ARG, "pool belongs to another context");
+// Loads a code object and resolves its kernels and their workgroup limits.
+int load_object(vk_ctx* ctx, const std::string& path, const std::vector<std::string>& names) {
+  FILE* fp = fopen(path.c_str(), "rb");
+  if (!fp) return fail(VK_ERR_NOT_WIRED, "code object %s not found (build the extension first)", path.c_str());
+  fclose(fp);
+  hipModule_t module = nullptr;
+  hipError_t e = hipModuleLoad(&module, path.c_str());
+  if (e != hipSuccess)
+    return fail(VK_ERR_NOT_WIRED, "hipModuleLoad(%s) failed: %s", path.c_str(), hipGetErrorString(e));
+  ctx->modules.push_back(module);
+  for (const auto& nm : names) {
+    hipFunction_t f = nullptr;
+    e = hipModuleGetFunction(&f, module, nm.c_str());
+    if (e != hipSuccess)
+      return fail(VK_ERR_NOT_WIRED, "kernel %s missing from %s: %s", nm.c_str(), path.c_str(), hipGetErrorString(e));
+    int max_threads = 0;
+    e = hipFuncGetAttribute(&max_threads, HIP_FUNC_ATTRIBUTE_MAX_THREADS_PER_BLOCK, f);
+    if (e != hipSuccess || max_threads <= 0)
+      return fail(VK_ERR_NOT_WIRED, "workgroup limit of kernel %s unreadable: %s", nm.c_str(), hipGetErrorString(e));
+    ctx->fns[nm] = f;
+    ctx->max_threads[nm] = max_threads;
+  }
   return VK_OK;
+}
+
+// Unloads a context's code objects and deletes it.
+void unload(vk_ctx* ctx) {
+  for (hipModule_t m : ctx->modules) hipModuleUnload(m);
+  delete ctx;
 }
 
 }  // namespace
@@ -295,20 +233,10 @@ extern "C" int vk_ctx_create(int device, const char* code_object_path, vk_ctx** 
   if (arch != "gfx950")
     return fail(VK_ERR_UNSUPPORTED, "device %d is %s; the code object is built for gfx950", device, arch.c_str());
 
-  const std::string path = code_object_path ? std::string(code_object_path) : default_code_object_path();
-  FILE* fp = fopen(path.c_str(), "rb");
-  if (!fp) return fail(VK_ERR_NOT_WIRED, "code object %s not found (build the extension first)", path.c_str());
-  fclose(fp);
-
   auto* ctx = new vk_ctx();
   ctx->device = device;
   ctx->arch = arch;
   ctx->n_cu = prop.multiProcessorCount;
-  e = hipModuleLoad(&ctx->module, path.c_str());
-  if (e != hipSuccess) {
-    delete ctx;
-    return fail(VK_ERR_NOT_WIRED, "hipModuleLoad(%s) failed: %s", path.c_str(), hipGetErrorString(e));
-  }
   std::vector<std::string> names(std::begin(kKernelNames), std::end(kKernelNames));
   for (int kv = 0; kv < 4; ++kv) {  // the runtime-group-size ("_gx") kernels
     for (int qt : {VK_DT_F16, VK_DT_F32}) {
@@ -348,30 +276,18 @@ extern "C" int vk_ctx_create(int device, const char* code_object_path, vk_ctx** 
       if (kv == VK_KV_F16 || kv == VK_KV_I8_BLK)
         for (int qt = 0; qt < 2; ++qt) names.push_back(tree_pfx_name(kv, g, qt));
     }
-  for (const auto& nm : names) {
-    hipFunction_t f = nullptr;
-    e = hipModuleGetFunction(&f, ctx->module, nm.c_str());
-    if (e != hipSuccess) {
-      hipModuleUnload(ctx->module);
-      delete ctx;
-      return fail(VK_ERR_NOT_WIRED, "kernel %s missing from %s: %s", nm.c_str(), path.c_str(), hipGetErrorString(e));
-    }
-    int max_threads = 0;
-    e = hipFuncGetAttribute(&max_threads, HIP_FUNC_ATTRIBUTE_MAX_THREADS_PER_BLOCK, f);
-    if (e != hipSuccess || max_threads <= 0) {
-      hipModuleUnload(ctx->module);
-      delete ctx;
-      return fail(VK_ERR_NOT_WIRED, "workgroup limit of kernel %s unreadable: %s", nm.c_str(), hipGetErrorString(e));
-    }
-    ctx->fns[nm] = f;
-    ctx->max_threads[nm] = max_threads;
+  int rc = load_object(ctx, code_object_path ? std::string(code_object_path) : beside_library("velokv_gfx950.co"), names);
+  if (!rc) rc = load_object(ctx, beside_library("velokv_sparse_gfx950.co"), sparse_kernel_names());
+  if (!rc) rc = load_object(ctx, beside_library("velokv_logits_gfx950.co"), logits_kernel_names());
+  if (rc) {
+    unload(ctx);
+    return rc;
   }
   e = hipMalloc(reinterpret_cast<void**>(&ctx->err_word), 256);
   if (e == hipSuccess) e = hipMemset(ctx->err_word, 0, 256);
   if (e != hipSuccess) {
     if (ctx->err_word) hipFree(ctx->err_word);
-    hipModuleUnload(ctx->module);
-    delete ctx;
+    unload(ctx);
     return fail(VK_ERR_HIP, "error word allocation failed: %s", hipGetErrorString(e));
   }
   // the no-alloc entry point's scratch: a failure here fails that entry point
@@ -392,8 +308,7 @@ extern "C" int vk_ctx_destroy(vk_ctx* ctx) {
   if (ctx->ws) hipFree(ctx->ws);
   for (void* p : ctx->ws_retired) hipFree(p);
   if (ctx->err_word) hipFree(ctx->err_word);
-  if (ctx->module) hipModuleUnload(ctx->module);
-  delete ctx;
+  unload(ctx);
   return VK_OK;
 }
 
@@ -735,11 +650,7 @@ extern "C" uint64_t vk_workspace_grow_bytes(uint64_t cur, uint64_t need) {
   return align_up(std::max(need, twice), 256);
 }
 
-namespace {
-
-// Split-K workspace: the caller's buffer when given (and large enough), else the
-// context's own, grown on demand.
-int split_workspace(vk_ctx* ctx, void* given, uint64_t given_bytes, uint64_t need, uint8_t** out) {
+int velokv::split_workspace(vk_ctx* ctx, void* given, uint64_t given_bytes, uint64_t need, uint8_t** out) {
   if (given) {
     if (given_bytes < need)
       return fail(VK_ERR_BAD_ARG, "workspace of %llu bytes, need %llu", (unsigned long long)given_bytes,
@@ -761,9 +672,7 @@ int split_workspace(vk_ctx* ctx, void* given, uint64_t given_bytes, uint64_t nee
   return VK_OK;
 }
 
-// Whether a call can have `need` bytes of scratch: in the buffer given, or in the
-// context's own, which may grow unless the stream is being captured.
-bool scratch_at_hand(vk_ctx* ctx, const void* given, uint64_t given_bytes, uint64_t need, void* stream) {
+bool velokv::scratch_at_hand(vk_ctx* ctx, const void* given, uint64_t given_bytes, uint64_t need, void* stream) {
   if (given) return given_bytes >= need;
   {
     std::lock_guard<std::mutex> lk(ctx->ws_mu);
@@ -773,6 +682,8 @@ bool scratch_at_hand(vk_ctx* ctx, const void* given, uint64_t given_bytes, uint6
   return !stream || (hipStreamIsCapturing(reinterpret_cast<hipStream_t>(stream), &st) == hipSuccess &&
                      st == hipStreamCaptureStatusNone);
 }
+
+namespace {
 
 constexpr int kPkMaxSeqs = 256;  // sequences a vk_decode_pk_* workgroup ranks
 constexpr int kPkMaxRounds = 16; // items per vk_decode_pk_* workgroup

@@ -231,6 +231,90 @@ struct CommitParams {
 // Per-sequence status of a tree commit (include/velokv.h VK_COMMIT_*).
 enum CommitStatus : int32_t { COMMIT_OK = 0, COMMIT_BAD_ROW = 1, COMMIT_PAST_TABLE = 2, COMMIT_BAD_PAGE = 3 };
 
+// Key index (include/velokv.h vk_index_*): per page and KV head the codes of the
+// keys' lower bound, then of their upper bound, T (the tile width) of each, and one
+// scale.
+struct IndexUpdateParams {
+  const uint8_t* kc;        // K codes of the layer
+  const uint8_t* ks;        // K scales of the layer (or null)
+  int8_t* codes;            // [n_pages][Hkv][2][T]
+  float* scales;            // [n_pages][Hkv]
+  const int32_t* block_tables;
+  const int32_t* seq_rows;
+  const int32_t* first_tokens;  // [S] first new position, or null: 0
+  const int32_t* context_lens;
+  uint32_t* err;
+  uint32_t tile_bytes, stile_bytes, s_step;
+  int32_t bt_stride, bt_rows, n_seqs, n_kv_heads, n_pages, page_tiles;
+  int32_t max_pages;        // pages of a sequence in the grid
+  int32_t cap_tokens;       // longest context
+  int32_t wg0;              // the launch's first workgroup
+};
+struct IndexReadParams {
+  const int8_t* codes;
+  const float* scales;
+  const int32_t* pages;     // [n]
+  float* lower;             // [n][Hkv][io_hd]
+  float* upper;
+  uint32_t* err;
+  int64_t n_chunks;         // n * Hkv * io_hd / 4
+  int32_t n_kv_heads, n_pages, io_hd, tile_hd;
+};
+
+// Selection of pages by their bounds, and attention over listed pages.
+struct SelectParams {
+  const int8_t* codes;      // the layer's bounds
+  const float* scales;
+  const void* q;            // [S][H][io_hd] of q_dtype
+  int32_t* pages;           // [S][Hkv][n_list]
+  uint32_t* keys;           // [S][Hkv][max_pages] ordered scores
+  const int32_t* block_tables;
+  const int32_t* seq_rows;
+  const int32_t* context_lens;
+  uint32_t* err;
+  int32_t bt_stride, bt_rows, n_seqs, n_heads, n_kv_heads, n_pool_pages, page_tokens;
+  int32_t cap_tokens, max_pages, n_list, n_first, n_last, io_hd;
+  int32_t n_chunks;         // workgroups that share a (sequence, KV head)'s pages
+};
+struct SparseParams {
+  const uint8_t* kc;
+  const uint8_t* vc;
+  const uint8_t* ks;
+  const uint8_t* vs;
+  const void* q;            // [S][H][io_hd]
+  float* out;               // [S][H][io_hd]
+  const int32_t* pages;     // [S][Hkv][n_list]
+  float* part_acc;          // [S][H][n_splits][T]
+  float* part_ml;           // [S][H][n_splits][2]
+  const int32_t* block_tables;
+  const int32_t* seq_rows;
+  const int32_t* context_lens;
+  uint32_t* err;
+  uint32_t tile_bytes, stile_bytes;
+  int32_t bt_stride, bt_rows, n_seqs, n_heads, n_kv_heads, n_pages, page_tiles;
+  int32_t cap_tokens, n_list, io_hd;
+  int32_t n_splits, split_entries;  // units per (sequence, KV head), list entries of each (at most kSparseEntries)
+  float scale_log2;         // softmax scale * log2(e)
+};
+constexpr int kSparseEntries = 512;  // list entries a unit stages in LDS
+
+// Log probabilities: rows of logits in parts of part_len, and their join.
+struct LogprobParams {
+  const void* logits;       // [n_rows][row_stride] of the kernel's type
+  const int32_t* tokens;    // [n_rows][n_tokens]
+  float* token_logprobs;    // [n_rows][n_tokens]
+  float* entropy;           // [n_rows] or null
+  int32_t* top_ids;         // [n_rows][n_top]
+  float* top_logprobs;      // [n_rows][n_top]
+  float* part_sums;         // [n_rows][n_parts][4]: max, sum of e^(x - max), sum of e^(x - max) (x - max)
+  uint64_t* part_top;       // [n_rows][n_parts][n_top], largest first
+  int64_t row_stride;
+  int32_t n_rows, vocab, n_tokens, n_top, n_parts, part_len;
+  float scale;
+};
+constexpr int kMaxTop = 32;        // alternatives of a row
+constexpr int kMaxLogitParts = 32;  // parts of a row
+
 struct MergeParams {
   const float* part_acc;
   const float* part_ml;

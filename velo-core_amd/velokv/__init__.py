@@ -17,7 +17,7 @@ from ._capi import (  # noqa: F401
     MISUSE_PAGE_OUT_OF_POOL, MISUSE_BLK_SPLIT_RUN,
 )
 from .runtime import (  # noqa: F401
-    BlockManager, CacheLookup, CachedSequence, Context, DeviceBuffer, Event, HipMemoryRuntime, KvCacheType,
+    BlockManager, CacheLookup, CachedSequence, Context, DeviceBuffer, Event, HipMemoryRuntime, KeyIndex, KvCacheType,
     MemoryRuntimeConfig, Pool, RadixCache,
     SlotPool, Stream, kv_bytes_per_token_per_head, rope_table,
 )

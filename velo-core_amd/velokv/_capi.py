@@ -108,6 +108,23 @@ class NixlItem(C.Structure):
                 ("wire_offset", C.c_uint64)]
 
 
+class SparseArgs(C.Structure):
+    _fields_ = [("layer", C.c_int32), ("q", C.c_void_p), ("q_dtype", C.c_int32), ("out", C.c_void_p),
+                ("pages", C.c_void_p), ("n_pages", C.c_int32), ("n_first", C.c_int32), ("n_last", C.c_int32),
+                ("block_tables", C.c_void_p), ("bt_stride", C.c_int32), ("seq_rows", C.c_void_p),
+                ("context_lens", C.c_void_p), ("n_seqs", C.c_int32), ("n_heads", C.c_int32),
+                ("max_context_len", C.c_int32), ("scale", C.c_float), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64)]
+
+
+class LogprobArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("dtype", C.c_int32), ("row_stride", C.c_int64), ("n_rows", C.c_int32),
+                ("vocab", C.c_int32), ("scale", C.c_float), ("tokens", C.c_void_p), ("n_tokens", C.c_int32),
+                ("token_logprobs", C.c_void_p), ("entropy", C.c_void_p), ("top_ids", C.c_void_p),
+                ("top_logprobs", C.c_void_p), ("n_top", C.c_int32), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64)]
+
+
 P = C.c_void_p
 I32 = C.c_int32
 U32 = C.c_uint32
@@ -148,6 +165,17 @@ PROTOTYPES = {
     "vk_tree_verify_workspace": [P, C.POINTER(TreeArgs), C.POINTER(U64)],
     "vk_tree_verify_plan": [P, C.POINTER(TreeArgs), C.POINTER(TreePlan)],
     "vk_tree_verify": [P, P, C.POINTER(TreeArgs), P],
+    "vk_index_create": [P, P, PP],
+    "vk_index_destroy": [P],
+    "vk_index_bytes": [P, C.POINTER(U64)],
+    "vk_index_update": [P, P, I32, P, I32, P, P, P, I32, I32, I32, P],
+    "vk_index_read": [P, P, I32, P, I32, P, P, P],
+    "vk_sparse_workspace": [P, C.POINTER(SparseArgs), C.POINTER(U64)],
+    "vk_select_pages": [P, P, C.POINTER(SparseArgs), P],
+    "vk_sparse_decode": [P, P, C.POINTER(SparseArgs), P],
+    "vk_select_decode": [P, P, C.POINTER(SparseArgs), P],
+    "vk_token_logprobs": [P, C.POINTER(LogprobArgs), P],
+    "vk_token_logprobs_workspace": [P, C.POINTER(LogprobArgs), C.POINTER(U64)],
     "vk_tree_mask": [PI32, I32, PU32],
     "vk_copy_blocks": [P, P, PI32, I32, P],
     "vk_tree_commit": [P, P, I32, I32, P, I32, P, P, I32, P, I32, P, P],

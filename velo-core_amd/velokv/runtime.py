@@ -250,6 +250,74 @@ class Context:
                 "max_partitions": p.max_partitions, "workspace_bytes": p.workspace_bytes,
                 "merge_launch": bool(p.merge_launch)}
 
+    def index_update(self, index: "KeyIndex", layer: int, context_lens, n_seqs: int, max_context_len: int,
+                     first_tokens=None, max_tokens: int = 0, block_tables=None, bt_stride: int = 0, seq_rows=None,
+                     stream=None):
+        """vk_index_update: the bounds of the pages that hold positions first_tokens (None: 0) .. context_lens - 1."""
+        check(lib().vk_index_update(self.h, index.h, layer, _bptr(block_tables), bt_stride, _bptr(seq_rows),
+                                    _bptr(first_tokens), _bptr(context_lens), n_seqs, max_context_len, max_tokens,
+                                    _sptr(stream)))
+
+    def index_read(self, index: "KeyIndex", layer: int, pages, n_pages: int, lower, upper, stream=None):
+        """vk_index_read: lower and upper bounds of listed pages as fp32 [n_pages][n_kv_heads][head_dim]."""
+        check(lib().vk_index_read(self.h, index.h, layer, _bptr(pages), n_pages, _bptr(lower), _bptr(upper),
+                                  _sptr(stream)))
+
+    def select_pages(self, index: "KeyIndex", layer: int, q, q_dtype: int, pages, n_pages: int, context_lens,
+                     n_seqs: int, n_heads: int, max_context_len: int, n_first: int = 1, n_last: int = 1,
+                     block_tables=None, bt_stride: int = 0, seq_rows=None, workspace=None, workspace_bytes: int = 0,
+                     stream=None):
+        """vk_select_pages: the n_pages best pages of each (sequence, KV head) by their bounds, ascending, into
+        pages (int32 [n_seqs][n_kv_heads][n_pages], -1 after a list's end)."""
+        a = _capi.SparseArgs(layer, _bptr(q), q_dtype, None, _bptr(pages), n_pages, n_first, n_last,
+                             _bptr(block_tables), bt_stride, _bptr(seq_rows), _bptr(context_lens), n_seqs, n_heads,
+                             max_context_len, 0.0, _bptr(workspace), workspace_bytes)
+        check(lib().vk_select_pages(self.h, index.h, C.byref(a), _sptr(stream)))
+
+    def sparse_decode(self, pool: "Pool", layer: int, q, q_dtype: int, out, pages, n_pages: int, context_lens,
+                      n_seqs: int, n_heads: int, max_context_len: int, block_tables=None, bt_stride: int = 0,
+                      seq_rows=None, scale: float = 0.0, workspace=None, workspace_bytes: int = 0, stream=None):
+        """vk_sparse_decode: decode attention over the pages listed for each (sequence, KV head)."""
+        a = _capi.SparseArgs(layer, _bptr(q), q_dtype, _bptr(out), _bptr(pages), n_pages, 0, 0, _bptr(block_tables),
+                             bt_stride, _bptr(seq_rows), _bptr(context_lens), n_seqs, n_heads, max_context_len, scale,
+                             _bptr(workspace), workspace_bytes)
+        check(lib().vk_sparse_decode(self.h, pool.h, C.byref(a), _sptr(stream)))
+
+    def select_decode(self, index: "KeyIndex", layer: int, q, q_dtype: int, out, pages, n_pages: int, context_lens,
+                      n_seqs: int, n_heads: int, max_context_len: int, n_first: int = 1, n_last: int = 1,
+                      block_tables=None, bt_stride: int = 0, seq_rows=None, scale: float = 0.0, workspace=None,
+                      workspace_bytes: int = 0, stream=None):
+        """vk_select_decode: select_pages, then sparse_decode over its lists (which stay in pages)."""
+        a = _capi.SparseArgs(layer, _bptr(q), q_dtype, _bptr(out), _bptr(pages), n_pages, n_first, n_last,
+                             _bptr(block_tables), bt_stride, _bptr(seq_rows), _bptr(context_lens), n_seqs, n_heads,
+                             max_context_len, scale, _bptr(workspace), workspace_bytes)
+        check(lib().vk_select_decode(self.h, index.h, C.byref(a), _sptr(stream)))
+
+    def sparse_workspace_bytes(self, pool: "Pool", n_seqs, n_heads, max_context_len, n_pages, bt_stride=0,
+                               q_dtype=DT_F16) -> int:
+        """vk_sparse_workspace: scratch that select_pages, sparse_decode or select_decode needs at most."""
+        a = _capi.SparseArgs(0, None, q_dtype, None, None, n_pages, 0, 0, C.c_void_p(1) if bt_stride else None,
+                             bt_stride, None, None, n_seqs, n_heads, max_context_len, 0.0, None, 0)
+        n = C.c_uint64()
+        check(lib().vk_sparse_workspace(pool.h, C.byref(a), C.byref(n)))
+        return n.value
+
+    def token_logprobs(self, logits, dtype: int, n_rows: int, vocab: int, tokens=None, n_tokens: int = 0,
+                       token_logprobs=None, entropy=None, top_ids=None, top_logprobs=None, n_top: int = 0,
+                       row_stride: int = 0, scale: float = 0.0, workspace=None, workspace_bytes: int = 0, stream=None):
+        """vk_token_logprobs: log probabilities of given tokens, entropy and the n_top most probable tokens of
+        each row of logits."""
+        a = _capi.LogprobArgs(_bptr(logits), dtype, row_stride, n_rows, vocab, scale, _bptr(tokens), n_tokens,
+                              _bptr(token_logprobs), _bptr(entropy), _bptr(top_ids), _bptr(top_logprobs), n_top,
+                              _bptr(workspace), workspace_bytes)
+        check(lib().vk_token_logprobs(self.h, C.byref(a), _sptr(stream)))
+
+    def token_logprobs_workspace_bytes(self, n_rows: int, vocab: int, n_top: int = 0, dtype: int = DT_F16) -> int:
+        a = _capi.LogprobArgs(None, dtype, 0, n_rows, vocab, 0.0, None, 0, None, None, None, None, n_top, None, 0)
+        n = C.c_uint64()
+        check(lib().vk_token_logprobs_workspace(self.h, C.byref(a), C.byref(n)))
+        return n.value
+
     def copy_blocks(self, pool: "Pool", pairs, stream=None):
         p = np.ascontiguousarray(np.asarray(pairs, dtype=np.int32).reshape(-1))
         check(lib().vk_copy_blocks(self.h, pool.h, p.ctypes.data_as(C.POINTER(C.c_int32)), len(p) // 2,
@@ -500,6 +568,33 @@ class Pool:
                 a = np.ascontiguousarray(parts[key]).view(np.uint8).reshape(-1)
                 assert a.nbytes == n, (key, a.nbytes, n)
                 DeviceBuffer(self.ctx, n, ptr=ptr, owned=False).upload(a)
+
+
+class KeyIndex:
+    """Bounds of the keys of every page of a pool (vk_index_create), for select_pages."""
+
+    def __init__(self, ctx: Context, pool: Pool):
+        self.ctx, self.pool = ctx, pool  # the pool outlives its index
+        h = C.c_void_p()
+        self.h = h
+        check(lib().vk_index_create(ctx.h, pool.h, C.byref(h)))
+
+    def close(self):
+        if self.h:
+            lib().vk_index_destroy(self.h)
+            self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    @property
+    def nbytes(self) -> int:
+        n = C.c_uint64()
+        check(lib().vk_index_bytes(self.h, C.byref(n)))
+        return n.value
 
 
 class BlockManager:

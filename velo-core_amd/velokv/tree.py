@@ -23,8 +23,9 @@ class TreeNode:
 
 @dataclass
 class TreeVerifyResult:
-    """Target-model token per tree node (speculative.rs:36-40)."""
+    """Target-model token per tree node (speculative.rs:36-40), and its log probability where known."""
     expected: list[int]
+    logprobs: list[float] = field(default_factory=list)
 
 
 @dataclass
@@ -69,6 +70,17 @@ class SpeculativeTree:
                     best = path
                     rejected = verified.expected[i] if i < len(verified.expected) else None
         return best, rejected
+
+    def verify_logits(self, ctx, logits, dtype: int, vocab: int, row_stride: int = 0, stream=None) -> TreeVerifyResult:
+        """The target model's most probable token after each node, and its log probability, from device logits
+        [n_nodes][row_stride] (vk_token_logprobs): what find_best_path and best_path_nodes take
+        (verify_tree, speculative.rs:217-242). Waits for the stream."""
+        n = len(self.nodes)
+        ids, top = ctx.alloc(4 * n), ctx.alloc(4 * n)
+        ctx.token_logprobs(logits, dtype, n, vocab, top_ids=ids, top_logprobs=top, n_top=1, row_stride=row_stride,
+                           stream=stream)
+        ctx.sync(stream)
+        return TreeVerifyResult(ids.download((n,), np.int32).tolist(), top.download((n,), np.float32).tolist())
 
     def path_nodes(self, node_idx: int) -> list[int]:
         """Node indices from the root to node_idx (get_path, speculative.rs:81-94, as node indices)."""
