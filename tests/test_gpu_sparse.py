@@ -477,7 +477,7 @@ def test_captured_steps_replay(ctx):
         ctx.index_update(index, 0, stream=stream, **d)
         ctx.select_decode(index, 0, q, velokv.DT_F16, out, pages, 32, n_heads=8, workspace=ws, workspace_bytes=need, stream=stream, **d)
         with pytest.raises(velokv.VkError) as e:
-            fresh.select_decode(index2, 0, q, velokv.DT_F16, out, pages, 2, stream=stream, n_heads=8, context_lens=lens, n_seqs=2,
+            fresh.select_decode(index2, 0, q, velokv.DT_F16, out, pages, 700, stream=stream, n_heads=8, context_lens=lens, n_seqs=2,
                                 max_context_len=640, block_tables=d["block_tables"], bt_stride=40)
         assert "workspace" in str(e.value)
     for step in range(4):
@@ -523,7 +523,7 @@ def test_refusals(ctx):
                  lambda: ctx.index_update(index, 0, **dict(d, context_lens=None)),
                  lambda: ctx.index_read(index, 0, pages, 1, out.ptr + 4, out),
                  lambda: ctx.index_read(index, 0, pages, -1, out, out),
-                 lambda: ctx.select_pages(index, 0, workspace=pages, workspace_bytes=4, **good)):
+                 lambda: ctx.sparse_decode(c.pool, 0, out=out, workspace=pages, workspace_bytes=4, **dict(good, n_pages=700))):
         with pytest.raises(velokv.VkError) as e:
             call()
         assert e.value.code == velokv.ERR_BAD_ARG

@@ -33,6 +33,7 @@ DEV float dpp(float x) {
 }
 constexpr int DPP_QUAD_XOR1 = 0xB1;    // quad_perm [1,0,3,2]
 constexpr int DPP_QUAD_XOR2 = 0x4E;    // quad_perm [2,3,0,1]
+constexpr int DPP_ROW_ROR2 = 0x122;
 constexpr int DPP_ROW_ROR4 = 0x124;
 constexpr int DPP_ROW_ROR8 = 0x128;
 constexpr int DPP_ROW_HALF_MIRROR = 0x141;

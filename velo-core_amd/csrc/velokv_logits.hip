@@ -9,8 +9,8 @@ namespace {
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kLogitWaves = 4;
-constexpr int kLogitThreads = WAVE * kLogitWaves;
-constexpr int kList = 512;  // candidates of a wave
+constexpr int kList = 512;       // candidates of a wave
+constexpr int kStepValues = 32;  // values of a thread in a step
 
 // =============================================================================
 // Log probabilities of a row x (logits times scale): with M = max x,
@@ -20,8 +20,10 @@ constexpr int kList = 512;  // candidates of a wave
 // thread keeps its own running M, Z and T; a wave keeps a list of candidates for the
 // largest values. A candidate is one 64-bit word, the value as an ordered key above
 // the complement of its index, so that words differ and their order is the order
-// wanted. thr is a word that at least n_top of the wave's words reach: only larger
-// ones are added, and after the first vectors of a row few are.
+// wanted. In the first step a workgroup takes the n_top-th largest of the maxima of 32
+// groups of its lanes: at least n_top values reach it, and few more. Only those, and
+// later values above it, are candidates. A wave whose list they do not fit (equal or
+// rising values) works vector by vector with words of its own as the bound.
 // =============================================================================
 struct Sums { float m, z, t; };
 
@@ -47,8 +49,8 @@ DEV uint64_t word_of(float x, int index) {
 }
 DEV int word_index(uint64_t w) { return (int)~(uint32_t)w; }
 
-// The k-th largest of a wave's words (N a lane, 0 = none): the largest word that k of
-// them reach, found bit by bit; 0 where there are fewer than k.
+// A bound that exactly k of a wave's words (N a lane, 0 = none) reach, found bit by bit;
+// 0 where there are no more than k.
 template <int N>
 DEV uint64_t kth_word(const uint64_t (&x)[N], int k) {
   uint64_t best = 0;
@@ -58,6 +60,7 @@ DEV uint64_t kth_word(const uint64_t (&x)[N], int k) {
 #pragma unroll
     for (int i = 0; i < N; ++i) count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[i] >= t));
     if (count >= k) best = t;
+    if (count == k) break;
   }
   return best;
 }
@@ -95,7 +98,7 @@ DEV void write_row(const LogprobParams& P, int row, const Sums& s, const uint64_
   const float log_z = logf(s.z);
   const auto logprob = [&](float x) { return s.m == -kInf && s.z == 0.0f ? -kInf : (x - s.m) * P.scale - log_z; };
   const int tid = (int)threadIdx.x;
-  for (int i = tid; i < P.n_tokens; i += kLogitThreads) {
+  for (int i = tid; i < P.n_tokens; i += (int)blockDim.x) {
     const int64_t at = (int64_t)row * P.n_tokens + i;
     const int t = P.tokens[at];
     float x = -kInf;
@@ -115,70 +118,177 @@ DEV void write_row(const LogprobParams& P, int row, const Sums& s, const uint64_
 
 // Sorts words into top[0 .. k), largest first: each word's place is the number of larger ones.
 DEV void rank_words(const uint64_t* words, int n, int k, uint64_t* top) {
-  for (int i = (int)threadIdx.x; i < n; i += kLogitThreads) {
+  for (int i = (int)threadIdx.x; i < n; i += (int)blockDim.x) {
     const uint64_t x = words[i];
     int place = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) place += words[j] > x;
     if (place < k) top[place] = x;
   }
 }
 
+// One workgroup of W waves per (row, part). DT: the logits' type.
 template <int DT>
 DEV void logprob_part(const LogprobParams& P) {
   constexpr int ESZ = DT == DT_F32 ? 4 : 2;
-  constexpr int EPV = 16 / ESZ;     // values of a 16-byte vector
-  constexpr int NV = 32 / EPV;      // vectors of a thread in a step
-  __shared__ uint64_t lists[kLogitWaves][kList];
-  __shared__ uint64_t words[kLogitWaves * kMaxTop];
+  constexpr int EPV = 16 / ESZ;             // values of a 16-byte vector
+  constexpr int NV = kStepValues / EPV;     // vectors of a thread in a step
+  constexpr int W = kLogitWaves, THREADS = W * WAVE;
+  constexpr int GROUPS = 32 / W;            // groups of a wave's lanes
+  __shared__ uint64_t lists[W][kList];
+  __shared__ uint64_t words[W * kMaxTop];
   __shared__ uint64_t top[kMaxTop];
-  __shared__ float sums[kLogitWaves][3];
-  __shared__ int counts[kLogitWaves];
+  __shared__ float sums[W][3], group_max[32];
+  __shared__ int counts[W];
   const int tid = (int)threadIdx.x, lane = lane_id(), w = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int row = (int)(blockIdx.x / P.n_parts), part = (int)(blockIdx.x % P.n_parts);
   const int k = P.n_top;
   const float c = P.scale * kLog2e;
   const uint8_t* base = reinterpret_cast<const uint8_t*>(P.logits) + (int64_t)row * P.row_stride * ESZ;
-  // vectors are aligned: vector i holds values i EPV - off .. of the row; the values of
-  // this part are [begin, end)
+  // vectors are aligned: vector i holds values i EPV - off .. of the row. The values of
+  // this part are [begin, end): the whole vectors [v_begin, v_end), and less than two
+  // vectors of values beside them, one each for the first threads
   const int off = (int)(reinterpret_cast<uint64_t>(base) & 15) / ESZ;
   const int begin = part * P.part_len, end = min(P.vocab, begin + P.part_len);
-  const int v_begin = (begin + off) / EPV, v_end = (end + off + EPV - 1) / EPV;
+  const int v_begin = (begin + off + EPV - 1) / EPV, v_end = max(v_begin, (end + off) / EPV);
+  const int n_head = min(end, v_begin * EPV - off) - begin;
+  const int extra = tid < n_head ? begin + tid : v_end * EPV - off + tid - n_head;
+  const bool has_extra = extra < end && tid < 2 * EPV;
+  float x_extra = -kInf;
+  if (has_extra)
+    x_extra = DT == DT_F32 ? reinterpret_cast<const float*>(base)[extra] : h2f(reinterpret_cast<const uint16_t*>(base)[extra]);
 
+  // (no load sits in a branch: threads past the last vector load it again, and step()
+  // takes -infinity in its place)
   const auto load = [&](u32x4(&r)[NV], int v0) {
+    if (v_end == v_begin) return;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int v = v0 + i * kLogitThreads + tid, at = v * EPV - off;
-      if (at >= begin && at + EPV <= end) {
-        r[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(base + (int64_t)at * ESZ));
-      } else {  // the row's ends
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) {
-          uint32_t b = DT == DT_F32 ? 0xFF800000u : 0xFC00u;  // -infinity
-          if (v < v_end && at + e >= begin && at + e < end)
-            b = DT == DT_F32 ? reinterpret_cast<const uint32_t*>(base)[at + e] : reinterpret_cast<const uint16_t*>(base)[at + e];
-          if constexpr (DT == DT_F32) r[i][e] = b;
-          else r[i][e / 2] = e % 2 ? r[i][e / 2] | b << 16 : b;
-        }
-      }
+      const int v = min(v0 + i * THREADS + tid, v_end - 1);
+      r[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(base + ((int64_t)v * EPV - off) * ESZ));
     }
+  };
+  const auto value = [](const u32x4& r, int e) {
+    return DT == DT_F32 ? bitcast<float>(r[e]) : e % 2 ? half_hi(r[e / 2]) : half_lo(r[e / 2]);
   };
 
   Sums s{-kInf, 0.0f, 0.0f};
-  uint64_t thr = 0;
-  float thr_x = 0.0f;
-  int n = 0;
+  uint64_t thr = 0;      // candidates of later steps are larger words; 0: not known
+  float thr_x = -kInf;   // its value
+  int n = 0;             // candidates in the list
   uint64_t* list = lists[w];
-  const auto step = [&](const u32x4(&r)[NV], int v0) {
-    float x[NV][EPV], vmax[NV], m = -kInf;
+  // Adds one vector's words that can still be among the k largest of the wave's.
+  const auto take_words = [&](const uint64_t(&word)[EPV]) {
+    uint64_t most[1] = {0};
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      vmax[i] = -kInf;
+    for (int e = 0; e < EPV; ++e) most[0] = max(most[0], word[e]);
+    // words that reach a bound that k lanes' largest reach: at most one in each lane but
+    // those k, so (kMaxTop - 1) EPV + 1 are the most that the list needs room for
+    const uint64_t kth = max(kth_word(most, k), thr);
+    if (n > kList - kMaxTop * EPV) n = trim_list(list, n, k);
+    n = push_words(list, n, word, kth);
+    if (kth > thr) {
+      thr = kth;
+      thr_x = key_value((uint32_t)(thr >> 32));
+    }
+  };
+  const auto step = [&](u32x4(&r)[NV], int v0, bool first) {
+    if (v0 + NV * THREADS > v_end) {
 #pragma unroll
-      for (int e = 0; e < EPV; ++e) {
-        x[i][e] = DT == DT_F32 ? bitcast<float>(r[i][e]) : e % 2 ? half_hi(r[i][e / 2]) : half_lo(r[i][e / 2]);
-        vmax[i] = fmaxf(vmax[i], x[i][e]);
+      for (int i = 0; i < NV; ++i) {
+        const bool in = v0 + i * THREADS + tid < v_end;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[i][j] = in ? r[i][j] : DT == DT_F32 ? 0xFF800000u : 0xFC00FC00u;
       }
-      m = fmaxf(m, vmax[i]);
+    }
+    float mv = -kInf;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) mv = fmaxf(mv, value(r[i], e));
+    const float m = first ? fmaxf(mv, x_extra) : mv;
+    if (k > 0) {
+      bool all = false;  // whether the wave looks at each vector by itself
+      if (first) {
+        // the maxima of groups of 8 lanes, and the k-th of the 32 (the vectors' alone: values
+        // of later steps may come before the row's last ones, which are among the extra)
+        float gm = fmaxf(mv, dpp<DPP_QUAD_XOR1>(mv));
+        gm = fmaxf(gm, dpp<DPP_QUAD_XOR2>(gm));
+        gm = fmaxf(gm, dpp<DPP_ROW_HALF_MIRROR>(gm));
+        if (lane % (WAVE / GROUPS) == 0) group_max[w * GROUPS + lane / (WAVE / GROUPS)] = gm;
+        __syncthreads();
+        const float mine = group_max[lane & 31];
+        int place = 0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const float o = readlane_f(mine, j);
+          place += o > mine || (o == mine && j < lane);
+        }
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(lane < 32 && place == k - 1);
+        thr_x = readlane_f(mine, __builtin_ctzll(hit));
+      }
+      // candidates: at least thr_x in the first step, above it later
+      const bool any = first ? m >= thr_x : m > thr_x;
+      if (first && thr_x == -kInf) {
+        all = true;
+      } else if (__builtin_amdgcn_ballot_w64(any) != 0) {
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < EPV; ++e) {
+            const float x = value(r[i], e);
+            count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(first ? x >= thr_x : x > thr_x));
+          }
+        if (first) count += 2 * EPV;
+        all = n + count > kList;
+        if (!all) {
+          const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < EPV; ++e) {
+              const float x = value(r[i], e);
+              const bool in = first ? x >= thr_x : x > thr_x;
+              const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
+              if (mask == 0) continue;
+              if (in) list[n + __builtin_popcountll(mask & below)] = word_of(x, (v0 + i * THREADS + tid) * EPV - off + e);
+              n += __builtin_popcountll(mask);
+            }
+          if (first) {
+            const bool in = has_extra && x_extra >= thr_x;
+            const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
+            if (in) list[n + __builtin_popcountll(mask & below)] = word_of(x_extra, extra);
+            n += __builtin_popcountll(mask);
+          }
+        }
+      }
+      if (all) {
+        if (first) {
+          uint64_t word[EPV] = {};
+          word[0] = has_extra ? word_of(x_extra, extra) : 0;
+          take_words(word);
+          thr = 0;  // (the extra values are not the lowest: equal ones may still follow)
+        }
+#pragma unroll 1
+        for (int i = 0; i < NV; ++i) {
+          float vm = -kInf;
+          u32x4 rv = r[0];
+#pragma unroll
+          for (int j = 1; j < NV; ++j) rv = i == j ? r[j] : rv;
+#pragma unroll
+          for (int e = 0; e < EPV; ++e) vm = fmaxf(vm, value(rv, e));
+          if (__builtin_amdgcn_ballot_w64(thr == 0 || vm > thr_x) != 0) {
+            uint64_t word[EPV];
+            const int v = v0 + i * THREADS + tid;
+#pragma unroll
+            for (int e = 0; e < EPV; ++e) word[e] = v < v_end ? word_of(value(rv, e), v * EPV - off + e) : 0;
+            take_words(word);
+          }
+        }
+      } else if (first) {
+        thr = (uint64_t)(order_key(thr_x) + 1) << 32;  // any larger value, whatever its index
+      }
     }
     if (m > s.m) {
       const float f = __builtin_amdgcn_exp2f((s.m - m) * c);
@@ -191,42 +301,28 @@ DEV void logprob_part(const LogprobParams& P) {
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < EPV; ++e) {
-        const float d = x[i][e] - at, p = __builtin_amdgcn_exp2f(d * c);
+        const float d = value(r[i], e) - at, p = __builtin_amdgcn_exp2f(d * c);
         s.z += p;
-        s.t += p == 0.0f ? 0.0f : p * d;
+        s.t = fmaf(p, fmaxf(d, -3e38f), s.t);  // (p is 0 where d is -infinity)
       }
-    if (k == 0) return;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (__builtin_amdgcn_ballot_w64(thr == 0 || vmax[i] > thr_x) == 0) continue;
-      uint64_t word[EPV], most[1] = {0};
-      const int first = (v0 + i * kLogitThreads + tid) * EPV - off;
-#pragma unroll
-      for (int e = 0; e < EPV; ++e) {
-        word[e] = first + e >= begin && first + e < end ? word_of(x[i][e], first + e) : 0;
-        most[0] = word[e] > most[0] ? word[e] : most[0];
-      }
-      // fewer than k lanes hold a larger word than the k-th largest of the lanes' largest:
-      // at most (kMaxTop - 1) EPV + 1 words reach it
-      const uint64_t kth = kth_word(most, k);
-      if (n > kList - kMaxTop * EPV) n = trim_list(list, n, k);
-      n = push_words(list, n, word, max(kth, thr));
-      if (kth > thr) {
-        thr = kth;
-        thr_x = key_value((uint32_t)(thr >> 32));
-      }
+    if (first) {
+      const float d = x_extra - at, p = __builtin_amdgcn_exp2f(d * c);
+      s.z += p;
+      s.t = fmaf(p, fmaxf(d, -3e38f), s.t);
     }
   };
 
   u32x4 a[NV], b[NV];
-  constexpr int STEP = NV * kLogitThreads;
+  constexpr int STEP = NV * THREADS;
   load(a, v_begin);
-  for (int v = v_begin; v < v_end; v += 2 * STEP) {
-    load(b, v + STEP);
-    step(a, v);
+  load(b, v_begin + STEP);
+  step(a, v_begin, true);
+  for (int v = v_begin + STEP; v < v_end; v += 2 * STEP) {
+    load(a, v + STEP);
+    step(b, v, false);
     if (v + STEP >= v_end) break;
-    load(a, v + 2 * STEP);
-    step(b, v + STEP);
+    load(b, v + 2 * STEP);
+    step(a, v + STEP, false);
   }
 
   s = wave_join(s, c);
@@ -235,14 +331,16 @@ DEV void logprob_part(const LogprobParams& P) {
     if (n > kMaxTop) n = trim_list(list, n, k);
     if (lane == 0) counts[w] = n;
   }
+  if (tid < k) top[tid] = 0;
   __syncthreads();
-  s = Sums{sums[0][0], sums[0][1], sums[0][2]};
-  for (int i = 1; i < kLogitWaves; ++i) s = join(s, Sums{sums[i][0], sums[i][1], sums[i][2]}, c);
+  s = Sums{sums[lane % W][0], sums[lane % W][1], sums[lane % W][2]};
+#pragma unroll
+  for (int m = 1; m < W; m *= 2) s = join(s, Sums{shfl_xor(s.m, m), shfl_xor(s.z, m), shfl_xor(s.t, m)}, c);
   if (k > 0) {
     int at = 0, total = 0;
-    for (int i = 0; i < kLogitWaves; ++i) { at += i < w ? counts[i] : 0; total += counts[i]; }
+#pragma unroll
+    for (int i = 0; i < W; ++i) { at += i < w ? counts[i] : 0; total += counts[i]; }
     if (lane < n) words[at + lane] = list[lane];
-    if (tid < k) top[tid] = 0;
     __syncthreads();
     rank_words(words, total, k, top);
     __syncthreads();
@@ -263,19 +361,28 @@ DEV void logprob_join(const LogprobParams& P) {
   __shared__ uint64_t words[kMaxLogitParts * kMaxTop];
   __shared__ uint64_t top[kMaxTop];
   __shared__ int count;
-  const int tid = (int)threadIdx.x, row = (int)blockIdx.x, k = P.n_top, n = P.n_parts * k;
+  const int tid = (int)threadIdx.x, lane = lane_id(), row = (int)blockIdx.x, k = P.n_top, n = P.n_parts * k;
   const float c = P.scale * kLog2e;
-  const float4* parts = reinterpret_cast<const float4*>(P.part_sums) + (int64_t)row * P.n_parts;
-  Sums s{parts[0].x, parts[0].y, parts[0].z};
-  for (int i = 1; i < P.n_parts; ++i) s = join(s, Sums{parts[i].x, parts[i].y, parts[i].z}, c);
+  // every wave joins the sums by itself, one part a lane
+  static_assert(kMaxLogitParts <= WAVE, "a part a lane");
+  const bool in_part = lane < P.n_parts;
+  const float4 ps = reinterpret_cast<const float4*>(P.part_sums)[(int64_t)row * P.n_parts + (in_part ? lane : 0)];
+  const uint64_t* in = P.part_top + (int64_t)row * n;
+  uint64_t least = 1;  // 0: no word
   if (k > 0) {
-    const uint64_t* in = P.part_top + (int64_t)row * n;
-    uint64_t least = 1;  // 0: no word
-    for (int i = 0; i < P.n_parts; ++i) least = max(least, in[i * k + k - 1]);
+    if (in_part) least = max(least, in[lane * k + k - 1]);
     if (tid == 0) count = 0;
     if (tid < k) top[tid] = 0;
+  }
+  const Sums s = wave_join(in_part ? Sums{ps.x, ps.y, ps.z} : Sums{-kInf, 0.0f, 0.0f}, c);
+  if (k > 0) {
+#pragma unroll
+    for (int m = 1; m < WAVE; m *= 2) {
+      const uint64_t o = (uint64_t)(uint32_t)__shfl_xor((int)(least >> 32), m, WAVE) << 32 | (uint32_t)__shfl_xor((int)least, m, WAVE);
+      least = max(least, o);
+    }
     __syncthreads();
-    for (int i = tid; i < n; i += kLogitThreads) {
+    for (int i = tid; i < n; i += (int)blockDim.x) {
       const uint64_t x = in[i];
       if (x >= least) words[atomicAdd(&count, 1)] = x;
     }
@@ -288,7 +395,7 @@ DEV void logprob_join(const LogprobParams& P) {
 
 }  // namespace
 
-#define VK_LOGITS(DT)                                                                                                  \
-  extern "C" __global__ void __launch_bounds__(kLogitThreads) vk_logprob_part_q##DT(const LogprobParams P) { logprob_part<DT>(P); } \
-  extern "C" __global__ void __launch_bounds__(kLogitThreads) vk_logprob_join_q##DT(const LogprobParams P) { logprob_join<DT>(P); }
+#define VK_LOGITS(DT)                                                                                                             \
+  extern "C" __global__ void __launch_bounds__(WAVE* kLogitWaves) vk_logprob_part_q##DT(const LogprobParams P) { logprob_part<DT>(P); } \
+  extern "C" __global__ void __launch_bounds__(WAVE* kLogitWaves) vk_logprob_join_q##DT(const LogprobParams P) { logprob_join<DT>(P); }
 VK_LOGITS(0) VK_LOGITS(1)

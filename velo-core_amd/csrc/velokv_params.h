@@ -247,6 +247,7 @@ struct IndexUpdateParams {
   uint32_t tile_bytes, stile_bytes, s_step;
   int32_t bt_stride, bt_rows, n_seqs, n_kv_heads, n_pages, page_tiles;
   int32_t max_pages;        // pages of a sequence in the grid
+  int32_t seq_wgs;          // workgroups of a sequence
   int32_t cap_tokens;       // longest context
   int32_t wg0;              // the launch's first workgroup
 };
@@ -257,7 +258,7 @@ struct IndexReadParams {
   float* lower;             // [n][Hkv][io_hd]
   float* upper;
   uint32_t* err;
-  int64_t n_chunks;         // n * Hkv * io_hd / 4
+  uint32_t n_chunks;        // n * Hkv * io_hd / 4
   int32_t n_kv_heads, n_pages, io_hd, tile_hd;
 };
 
@@ -267,15 +268,17 @@ struct SelectParams {
   const float* scales;
   const void* q;            // [S][H][io_hd] of q_dtype
   int32_t* pages;           // [S][Hkv][n_list]
-  uint32_t* keys;           // [S][Hkv][max_pages] ordered scores
+  uint32_t* keys;           // [S][Hkv][max_pages] ordered scores (vk_page_scores, vk_page_topk)
   const int32_t* block_tables;
   const int32_t* seq_rows;
   const int32_t* context_lens;
   uint32_t* err;
   int32_t bt_stride, bt_rows, n_seqs, n_heads, n_kv_heads, n_pool_pages, page_tokens;
   int32_t cap_tokens, max_pages, n_list, n_first, n_last, io_hd;
-  int32_t n_chunks;         // workgroups that share a (sequence, KV head)'s pages
+  int32_t n_chunks;         // vk_page_scores: workgroups that share a (sequence, KV head)'s pages
 };
+constexpr int kSelWaves = 8;      // waves of a workgroup of the selection
+constexpr int kSelPages = 8192;   // pages whose scores vk_page_select holds in LDS
 struct SparseParams {
   const uint8_t* kc;
   const uint8_t* vc;

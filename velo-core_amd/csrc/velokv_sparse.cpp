@@ -27,8 +27,8 @@ bool narrow(const vk_pool* pool) { return pool->geom.head_dim == 64; }
 const char* d64(const vk_pool* pool) { return narrow(pool) ? "_d64" : ""; }
 std::string update_name(const vk_pool* pool) { return "vk_index_update_kv" + std::to_string(pool->desc.kv_type) + d64(pool); }
 std::string rows_tag(int group, int q_dtype) { return std::string(group > 16 ? "_r2_q" : "_r1_q") + std::to_string(q_dtype); }
-std::string scores_name(const vk_pool* pool, int group, int q_dtype) {
-  return std::string("vk_page_scores") + d64(pool) + rows_tag(group, q_dtype);
+std::string select_name(const char* stage, const vk_pool* pool, int group, int q_dtype) {
+  return stage + std::string(d64(pool)) + rows_tag(group, q_dtype);
 }
 std::string sparse_name(const vk_pool* pool, int group, int q_dtype) {
   return "vk_sparse_kv" + std::to_string(pool->desc.kv_type) + d64(pool) + rows_tag(group, q_dtype);
@@ -84,18 +84,22 @@ int plan_sparse(const vk_ctx* ctx, const vk_pool* pool, const vk_sparse_args* a,
   pl->units = (uint64_t)a->n_seqs * d.n_kv_heads;
   pl->max_pages = (int)(((int64_t)a->max_context_len + d.block_size - 1) / d.block_size);
   const int64_t units = std::max<int64_t>(1, (int64_t)pl->units);
-  // selection: about four workgroups a CU, of 64 pages at least
-  pl->n_chunks = (int)std::max<int64_t>(1, std::min<int64_t>((4 * ctx->n_cu + units - 1) / units, (pl->max_pages + 63) / 64));
-  pl->select_bytes = pl->max_pages > a->n_pages ? align_up(pl->units * pl->max_pages * sizeof(uint32_t), 256) : 0;
-  // attention: two workgroups of four waves a CU, of eight tiles at least
-  const int pt = pool->geom.page_tiles;
-  const int listed = std::max(1, std::min(a->n_pages, a->n_pages));
-  const int64_t want = (2 * ctx->n_cu + units - 1) / units;
-  const int64_t most = std::max<int64_t>(1, (int64_t)listed * pt / 8);
-  const int64_t entries = std::max<int64_t>(1, (listed + std::min(want, most) - 1) / std::min(want, most));
-  pl->waves = 4;
+  // selection: one workgroup per (sequence, KV head), or several and a second launch
+  pl->n_chunks = 0;
+  pl->select_bytes = 0;
+  if (pl->max_pages > kSelPages) {
+    constexpr int kChunk = 64 * kSelWaves;
+    pl->n_chunks = (int)std::max<int64_t>(1, std::min<int64_t>((2 * ctx->n_cu + units - 1) / units, (pl->max_pages + kChunk - 1) / kChunk));
+    pl->select_bytes = align_up(pl->units * pl->max_pages * sizeof(uint32_t), 256);
+  }
+  // attention: eight waves a CU (more do not fit beside their registers), in one workgroup
+  // per (sequence, KV head) where there are as many as CUs, in parts of the list else
+  const int pt = pool->geom.page_tiles, cus = ctx->n_cu;
+  pl->waves = units >= 2 * cus || pl->group > 16 ? 4 : 8;
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(cus / units, (int64_t)a->n_pages * pt / 8));
+  const int64_t entries = (a->n_pages + parts - 1) / parts;
   pl->split_entries = (int)std::min<int64_t>(entries, kSparseEntries);
-  pl->n_splits = (listed + pl->split_entries - 1) / pl->split_entries;
+  pl->n_splits = (a->n_pages + pl->split_entries - 1) / pl->split_entries;
   pl->acc_bytes = pl->ml_bytes = 0;
   if (pl->n_splits > 1) {
     const uint64_t rows = (uint64_t)a->n_seqs * a->n_heads * pl->n_splits;
@@ -103,7 +107,7 @@ int plan_sparse(const vk_ctx* ctx, const vk_pool* pool, const vk_sparse_args* a,
     pl->ml_bytes = align_up(rows * 2 * sizeof(float), 256);
   }
   const uint64_t rows = ((uint64_t)a->n_seqs * a->n_heads + 3) / 4;
-  if (std::max({pl->units * pl->n_chunks * 256, pl->units * pl->n_splits * 64 * pl->waves, rows * 256}) > kMaxThreads)
+  if (std::max({pl->units * std::max(1, pl->n_chunks) * 64 * kSelWaves, pl->units * pl->n_splits * 64 * pl->waves, rows * 256}) > kMaxThreads)
     return fail(VK_ERR_UNSUPPORTED, "grid too large");
   return VK_OK;
 }
@@ -134,10 +138,12 @@ int run_select(vk_ctx* ctx, vk_key_index* index, const vk_sparse_args* a, const 
   p.n_last = a->n_last;
   p.io_hd = pool->geom.io_hd;
   p.n_chunks = pl.n_chunks;
-  if (pl.select_bytes)
-    if (int rc = launch(ctx, scores_name(pool, pl.group, a->q_dtype).c_str(), dim3((unsigned)(pl.units * pl.n_chunks)), dim3(256), p, stream))
-      return rc;
-  return launch(ctx, "vk_page_topk", dim3((unsigned)pl.units), dim3(256), p, stream);
+  const dim3 threads(64 * kSelWaves), units((unsigned)pl.units);
+  if (!pl.n_chunks) return launch(ctx, select_name("vk_page_select", pool, pl.group, a->q_dtype).c_str(), units, threads, p, stream);
+  if (int rc = launch(ctx, select_name("vk_page_scores", pool, pl.group, a->q_dtype).c_str(),
+                      dim3((unsigned)(pl.units * pl.n_chunks)), threads, p, stream))
+    return rc;
+  return launch(ctx, "vk_page_topk", units, threads, p, stream);
 }
 
 int run_attend(vk_ctx* ctx, vk_pool* pool, const vk_sparse_args* a, const SparsePlan& pl, uint8_t* ws, void* stream) {
@@ -206,7 +212,7 @@ std::vector<std::string> velokv::sparse_kernel_names() {
     for (int kv = 0; kv < 4; ++kv) names.push_back("vk_index_update_kv" + std::to_string(kv) + w);
     for (int group : {16, 32})
       for (int qt : {VK_DT_F32, VK_DT_F16}) {
-        names.push_back(std::string("vk_page_scores") + w + rows_tag(group, qt));
+        for (const char* stage : {"vk_page_select", "vk_page_scores"}) names.push_back(stage + std::string(w) + rows_tag(group, qt));
         for (int kv = 0; kv < 4; ++kv) names.push_back("vk_sparse_kv" + std::to_string(kv) + w + rows_tag(group, qt));
       }
   }
@@ -299,8 +305,9 @@ extern "C" int vk_index_update(vk_ctx* ctx, vk_key_index* index, int32_t layer, 
   constexpr int kWaves = 4;
   constexpr int64_t kMaxWgs = 1 << 23;  // launches of less than 2^32 threads
   const std::string name = update_name(pool);
-  const int64_t units = (int64_t)n_seqs * p.max_pages * p.n_kv_heads, wgs = (units + kWaves - 1) / kWaves;
-  if (wgs > 0x7FFFFFFF) return fail(VK_ERR_UNSUPPORTED, "grid too large");
+  const int64_t units = (int64_t)p.max_pages * p.n_kv_heads, seq_wgs = (units + kWaves - 1) / kWaves, wgs = seq_wgs * n_seqs;
+  if (units > 0x7FFFFFFF - kWaves || wgs > 0x7FFFFFFF) return fail(VK_ERR_UNSUPPORTED, "grid too large");
+  p.seq_wgs = (int32_t)seq_wgs;
   for (int64_t w = 0; w < wgs; w += kMaxWgs) {
     p.wg0 = (int32_t)w;
     if ((rc = launch(ctx, name.c_str(), dim3((unsigned)std::min(kMaxWgs, wgs - w)), dim3(64 * kWaves), p, stream))) return rc;
@@ -331,9 +338,10 @@ extern "C" int vk_index_read(vk_ctx* ctx, vk_key_index* index, int32_t layer, co
   p.n_pages = pool->desc.n_blocks;
   p.io_hd = pool->geom.io_hd;
   p.tile_hd = pool->geom.head_dim;
-  p.n_chunks = (int64_t)n_pages * p.n_kv_heads * (p.io_hd / 4);
-  if ((uint64_t)p.n_chunks > kMaxThreads - 255) return fail(VK_ERR_UNSUPPORTED, "grid too large");
-  return launch(ctx, "vk_index_read", dim3((unsigned)((p.n_chunks + 255) / 256)), dim3(256), p, stream);
+  const uint64_t chunks = (uint64_t)n_pages * p.n_kv_heads * (p.io_hd / 4);
+  if (chunks > kMaxThreads - 255) return fail(VK_ERR_UNSUPPORTED, "grid too large");
+  p.n_chunks = (uint32_t)chunks;
+  return launch(ctx, "vk_index_read", dim3((unsigned)((chunks + 255) / 256)), dim3(256), p, stream);
 }
 
 extern "C" int vk_sparse_workspace(const vk_pool* pool, const vk_sparse_args* a, uint64_t* bytes) {

@@ -7,6 +7,7 @@
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef short short2v __attribute__((ext_vector_type(2)));
 
 namespace {
 
@@ -33,25 +34,96 @@ DEV int to_code(float x, float inv) { return (int)fminf(fmaxf(rintf(x * inv), -1
 // A page with a key that is not finite has the scale infinity (it is chosen before
 // any other).
 // =============================================================================
+// Exchanges x's lanes with bit M set and y's without: afterwards a lane without it
+// holds both halves of x, one with it both of y.
+template <int M>
+DEV void swap_lanes(uint32_t& x, uint32_t& y) {
+  const auto r = M == 32 ? __builtin_amdgcn_permlane32_swap(x, y, false, false) : __builtin_amdgcn_permlane16_swap(x, y, false, false);
+  x = r[0];
+  y = r[1];
+}
+template <int M>
+DEV void swap_lanes(float& x, float& y) {
+  uint32_t a = bitcast<uint32_t>(x), b = bitcast<uint32_t>(y);
+  swap_lanes<M>(a, b);
+  x = bitcast<float>(a);
+  y = bitcast<float>(b);
+}
+template <int CTRL>
+DEV uint32_t dpp_u(uint32_t x, uint32_t old) { return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)x, CTRL, 0xF, 0xF, false); }
+
+// Bounds of dims as signed integers, one (fp32) or two (PK: 16 bits each) a word.
+// Integers take one instruction a comparison; a float minimum of a value from another
+// lane takes two.
+template <bool PK>
+DEV uint32_t word_min(uint32_t a, uint32_t b) {
+  if constexpr (PK) return bitcast<uint32_t>(__builtin_elementwise_min(bitcast<short2v>(a), bitcast<short2v>(b)));
+  else return (uint32_t)min((int)a, (int)b);
+}
+template <bool PK>
+DEV uint32_t word_max(uint32_t a, uint32_t b) {
+  if constexpr (PK) return bitcast<uint32_t>(__builtin_elementwise_max(bitcast<short2v>(a), bitcast<short2v>(b)));
+  else return (uint32_t)max((int)a, (int)b);
+}
+// A float's bits as an integer of the same order, NaN beyond infinity, and back (the map
+// is its own inverse).
+DEV uint32_t ordered_f32(uint32_t x) { return x ^ (uint32_t)((int)x >> 31) >> 1; }
+DEV uint32_t ordered_f16x2(uint32_t x) {
+  const short2v s = bitcast<short2v>(x);
+  return x ^ (bitcast<uint32_t>(s >> (short)15) & 0x7FFF7FFFu);
+}
+// Joins lanes l and l ^ M: lanes with bit M clear are left the first half of the N
+// words, the others the second, in [0, N / 2).
+template <bool PK, int N, int M>
+DEV void fold_lanes(uint32_t* lo, uint32_t* hi) {
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    swap_lanes<M>(lo[i], lo[i + N / 2]);
+    swap_lanes<M>(hi[i], hi[i + N / 2]);
+    lo[i] = word_min<PK>(lo[i], lo[i + N / 2]);
+    hi[i] = word_max<PK>(hi[i], hi[i + N / 2]);
+  }
+}
+// Over the lanes of a row of 16 that are equal mod LPT.
+template <bool PK, int CTRL, int N>
+DEV void join_turned(uint32_t* lo, uint32_t* hi) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    lo[i] = word_min<PK>(lo[i], dpp_u<CTRL>(lo[i], lo[i]));
+    hi[i] = word_max<PK>(hi[i], dpp_u<CTRL>(hi[i], hi[i]));
+  }
+}
+template <bool PK, int LPT, int N>
+DEV void join_row(uint32_t* lo, uint32_t* hi) {
+  if constexpr (LPT <= 8) join_turned<PK, DPP_ROW_ROR8, N>(lo, hi);
+  if constexpr (LPT <= 4) join_turned<PK, DPP_ROW_ROR4, N>(lo, hi);
+  if constexpr (LPT <= 2) join_turned<PK, DPP_ROW_ROR2, N>(lo, hi);
+}
+
+constexpr int kUpdateThreads = 256;
+
 template <int KV, int T>
 DEV void index_update(const IndexUpdateParams& P) {
   constexpr int ESZ = Esz<KV>::v;
+  constexpr bool I8 = ESZ == 1, BLK = KV == KV_I8_BLK, REF = KV == KV_I8_REF;
+  constexpr bool PK = KV == KV_F16 || BLK;           // two dims a word
   constexpr int EPC = 16 / ESZ;                      // dims of a 16-byte chunk
-  constexpr bool I8 = ESZ == 1;
   constexpr int LPT = I8 ? T / 32 : T / EPC;         // lanes that hold one token's chunks of a load
   constexpr int NI = 16 * T * ESZ / 1024;            // loads of 64 chunks per tile
   constexpr int NS = (I8 && T == 128) ? 2 : 1;       // sets of dims a lane holds
-  constexpr int TLANES = (I8 && T == 64) ? 32 : 64;  // lanes l and l ^ 32 hold the same dims
+  constexpr int NW = NS * EPC / (PK ? 2 : 1);        // words a lane holds
+  constexpr bool R16 = LPT <= 16, R32 = !(I8 && T == 64);  // lanes 16 (32) apart hold the same dims
+  constexpr int N1 = R32 ? NW / 2 : NW, NF = R16 ? N1 / 2 : N1;  // words left after each exchange
+  constexpr int NO = NF * (PK ? 2 : 1);              // dims a lane is left with, side by side
   const int lane = lane_id();
-  const int64_t unit = ((int64_t)P.wg0 + blockIdx.x) * (blockDim.x / WAVE) + threadIdx.x / WAVE;
-  const int kvh = (int)(unit % P.n_kv_heads);
-  const int64_t rest = unit / P.n_kv_heads;
-  const int s = (int)(rest / P.max_pages);
-  if (s >= P.n_seqs) return;
+  const int wg = P.wg0 + (int)blockIdx.x, s = wg / P.seq_wgs;
+  const int unit = (wg - s * P.seq_wgs) * (kUpdateThreads / WAVE) + __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE);
+  const int nth = unit / P.n_kv_heads, kvh = unit - nth * P.n_kv_heads;
+  if (nth >= P.max_pages) return;
   const int ctx = max(0, min(P.context_lens[s], P.cap_tokens));
   const int first = P.first_tokens ? max(0, P.first_tokens[s]) : 0;
   const int ptok = 16 * P.page_tiles;
-  const int64_t col = first / ptok + rest % P.max_pages;
+  const int64_t col = (int64_t)(first / ptok) + nth;
   if (first >= ctx || col * ptok >= ctx) return;
   const int page = P.block_tables[(int64_t)table_row(P.seq_rows, s, P.bt_rows) * P.bt_stride + col];
   if (page < 0 || page >= P.n_pages) {
@@ -61,11 +133,41 @@ DEV void index_update(const IndexUpdateParams& P) {
   const int nt = min(ptok, ctx - (int)col * ptok);
   const int tok = I8 ? (T == 128 ? lane >> 2 : (lane >> 1) & 15) : lane / LPT;  // of a load
 
-  float lo[NS][EPC], hi[NS][EPC], bad = 0.0f;
+  constexpr uint32_t kLeast = PK ? 0x80008000u : 0x80000000u, kMost = PK ? 0x7FFF7FFFu : 0x7FFFFFFFu;
+  uint32_t lo[NW], hi[NW];
+  float flo[NO], fhi[NO];
+  bool ok = true;  // every key is finite
 #pragma unroll
-  for (int n = 0; n < NS; ++n)
+  for (int d = 0; d < NO; ++d) { flo[d] = kInf; fhi[d] = -kInf; }
+  const auto clear = [&] {
 #pragma unroll
-    for (int e = 0; e < EPC; ++e) { lo[n][e] = kInf; hi[n][e] = -kInf; }
+    for (int i = 0; i < NW; ++i) { lo[i] = kMost; hi[i] = kLeast; }
+  };
+  // the tokens' lanes joined, and the lane's dims as floats
+  const auto join = [&](float scale) {
+    if constexpr (R32) fold_lanes<PK, NW, 32>(lo, hi);
+    if constexpr (R16) fold_lanes<PK, N1, 16>(lo, hi);
+    join_row<PK, LPT, NF>(lo, hi);
+#pragma unroll
+    for (int side = 0; side < 2; ++side)
+#pragma unroll
+      for (int i = 0; i < NF; ++i) {
+        const uint32_t w = side ? hi[i] : lo[i];
+        float* f = side ? fhi : flo;
+        const auto take = [&](int d, float x) { f[d] = side ? fmaxf(f[d], x) : fminf(f[d], x); };
+        if constexpr (BLK) {  // words of the even, then of the odd dims of four
+          take(4 * (i / 2) + i % 2, (float)((int)(w << 16) >> 24) * scale);
+          take(4 * (i / 2) + i % 2 + 2, (float)((int)w >> 24) * scale);
+        } else if constexpr (PK) {
+          const uint32_t x = ordered_f16x2(w);
+          f[2 * i] = half_lo(x);
+          f[2 * i + 1] = half_hi(x);
+        } else {
+          f[i] = bitcast<float>(ordered_f32(w));
+        }
+      }
+  };
+  clear();
   for (int t = 0; t * BS < nt; ++t) {
     const int64_t tile = ((int64_t)page * P.page_tiles + t) * P.n_kv_heads + kvh;
     const uint8_t* base = P.kc + tile * P.tile_bytes;
@@ -73,72 +175,81 @@ DEV void index_update(const IndexUpdateParams& P) {
 #pragma unroll
     for (int j = 0; j < NI; ++j) c[j] = *reinterpret_cast<const u32x4*>(base + 1024 * j + 16 * lane);
     float scale = 1.0f;
-    if constexpr (KV == KV_I8_BLK) scale = half_lo(*reinterpret_cast<const uint32_t*>(P.ks + tile * kBlkScaleStep));
-    if constexpr (KV == KV_I8_REF) scale = reinterpret_cast<const float*>(P.ks + tile * P.stile_bytes)[tok];
+    if constexpr (BLK) scale = half_lo(*reinterpret_cast<const uint32_t*>(P.ks + tile * kBlkScaleStep));
+    if constexpr (REF) scale = reinterpret_cast<const float*>(P.ks + tile * P.stile_bytes)[tok];
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
-      const int n = NS == 2 ? j : 0;
-      const int at = t * BS + (I8 ? tok : j * (WAVE / LPT) + tok);
-      if (at < nt) {
+      const int w0 = NS == 2 ? j * (NW / 2) : 0;
+      const bool in = t * BS + (I8 ? tok : j * (WAVE / LPT) + tok) < nt;
 #pragma unroll
-        for (int e = 0; e < EPC; ++e) {
-          float x;
-          if constexpr (I8) x = byte_to_f(c[j][e / 4], e % 4) * scale;
-          else if constexpr (KV == KV_F16) x = e % 2 ? half_hi(c[j][e / 2]) : half_lo(c[j][e / 2]);
-          else x = bitcast<float>(c[j][e]);
-          lo[n][e] = fminf(lo[n][e], x);
-          hi[n][e] = fmaxf(hi[n][e], x);
-          bad = fmaf(x, 0.0f, bad);
-        }
+      for (int i = 0; i < NW / NS; ++i) {
+        uint32_t x;
+        if constexpr (BLK) x = i % 2 ? c[j][i / 2] : bitcast<uint32_t>(bitcast<short2v>(c[j][i / 2]) << (short)8);  // codes in the high bytes
+        else if constexpr (REF) x = ordered_f32(bitcast<uint32_t>(byte_to_f(c[j][i / 4], i % 4) * scale));
+        else if constexpr (PK) x = ordered_f16x2(c[j][i]);
+        else x = ordered_f32(c[j][i]);
+        lo[w0 + i] = word_min<PK>(lo[w0 + i], in ? x : kMost);
+        hi[w0 + i] = word_max<PK>(hi[w0 + i], in ? x : kLeast);
       }
+    }
+    if constexpr (BLK) {  // a scale a tile
+      ok = ok && finite(scale);
+      join(scale);
+      clear();
     }
   }
-  // the lanes of one set of dims: all that differ in the token
+  if constexpr (!BLK) join(1.0f);
   float top = 0.0f;
 #pragma unroll
-  for (int n = 0; n < NS; ++n)
-#pragma unroll
-    for (int e = 0; e < EPC; ++e) {
-#pragma unroll
-      for (int m = LPT; m < TLANES; m *= 2) {
-        lo[n][e] = fminf(lo[n][e], shfl_xor(lo[n][e], m));
-        hi[n][e] = fmaxf(hi[n][e], shfl_xor(hi[n][e], m));
-      }
-      top = fmaxf(top, fmaxf(fabsf(lo[n][e]), fabsf(hi[n][e])));
-    }
+  for (int d = 0; d < NO; ++d) {
+    top = fmaxf(top, fmaxf(fabsf(flo[d]), fabsf(fhi[d])));
+    ok = ok && finite(flo[d]) && finite(fhi[d]);
+  }
   top = wave_max(top);
-  const bool ok = __builtin_amdgcn_ballot_w64(!(bad == 0.0f)) == 0;
+  ok = __builtin_amdgcn_ballot_w64(!ok) == 0;
   const float inv = ok ? code_scale(top) : 0.0f;
   const int64_t at = (int64_t)page * P.n_kv_heads + kvh;
-  int8_t* codes = P.codes + at * 2 * T;
-  // tokens 0's lanes write the lower bounds, tokens 1's the upper ones
-  if (tok < 2) {
+  // the first dim of the lane's: of its chunk, then the half that an exchange left it
+  int dim = I8 ? (T == 128 ? 32 * (lane & 3) : 32 * (lane & 1) + 16 * (lane >> 5)) : EPC * (lane % LPT);
+  if constexpr (R32) dim += (lane >> 5) * (N1 * (PK ? 2 : 1));
+  if constexpr (R16) dim += ((lane >> 4) & 1) * NO;
+  // of a row's lanes that hold the same dims the first writes the lower bounds and the
+  // second the upper; where there is one (LPT >= 16) it writes both
+  constexpr int WL = LPT < 16 ? LPT : 16;
+  const int copy = (lane & 15) / WL;
+  const auto write = [&](const float(&f)[NO], int8_t* dst) {
+    uint32_t w[(NO + 3) / 4] = {};
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      const int dim = I8 ? (T == 128 ? 32 * (lane & 3) + 16 * n : 32 * (lane & 1) + 16 * (lane >> 5)) : EPC * (lane % LPT);
-      uint32_t w[EPC / 4];
+    for (int d = 0; d < NO; ++d) w[d / 4] |= ((uint32_t)to_code(f[d], inv) & 0xFFu) << (8 * (d % 4));
+    if constexpr (NO == 1) {
+      *dst = (int8_t)w[0];
+    } else if constexpr (NO == 2) {
+      *reinterpret_cast<uint16_t*>(dst) = (uint16_t)w[0];
+    } else {
 #pragma unroll
-      for (int e = 0; e < EPC; ++e) {
-        const uint32_t b = (uint32_t)to_code(tok == 0 ? lo[n][e] : hi[n][e], inv) & 0xFFu;
-        w[e / 4] = e % 4 ? w[e / 4] | b << (8 * (e % 4)) : b;
-      }
-      uint32_t* dst = reinterpret_cast<uint32_t*>(codes + tok * T + dim);
-#pragma unroll
-      for (int i = 0; i < EPC / 4; ++i) dst[i] = w[i];
+      for (int i = 0; i < NO / 4; ++i) reinterpret_cast<uint32_t*>(dst)[i] = w[i];
     }
+  };
+  int8_t* codes = P.codes + at * 2 * T + dim;
+  if constexpr (WL == 16) {
+    write(flo, codes);
+    write(fhi, codes + T);
+  } else if (copy < 2) {
+    float f[NO];
+#pragma unroll
+    for (int d = 0; d < NO; ++d) f[d] = copy ? fhi[d] : flo[d];
+    write(f, codes + copy * T);
   }
   if (lane == 0) P.scales[at] = ok ? top / 127.0f : kInf;
 }
 
 // The bounds of listed pages as fp32: four dims a thread.
 DEV void index_read(const IndexReadParams& P) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= P.n_chunks) return;
-  const int per = P.io_hd / 4;
-  const int64_t row = i / per;
-  const int dim = (int)(i - row * per) * 4;
-  const int kvh = (int)(row % P.n_kv_heads);
-  const int page = P.pages[row / P.n_kv_heads];
+  const uint32_t per = (uint32_t)P.io_hd / 4, row = i / per, at_page = row / (uint32_t)P.n_kv_heads;
+  const int dim = (int)(i - row * per) * 4, kvh = (int)(row - at_page * (uint32_t)P.n_kv_heads);
+  const int page = P.pages[at_page];
   float4 lo = make_float4(0, 0, 0, 0), hi = lo;
   if (page < 0 || page >= P.n_pages) {
     flag_misuse(P.err, MISUSE_PAGE_OUT_OF_POOL);
@@ -168,25 +279,45 @@ DEV void index_read(const IndexReadParams& P) {
 // has the same bits however it is computed. Scores are kept as ordered 32-bit keys
 // (larger key = chosen earlier); the pages that are always kept have the largest.
 // =============================================================================
-constexpr int kSelWaves = 4;
-constexpr uint32_t kKeyKept = 0xFFFFFFFFu;
+//
+// The pages that are always kept are not scored. Where a (sequence, KV head)'s scores
+// fit LDS one workgroup computes them and selects (vk_page_select); longer contexts,
+// and long ones of few sequences, are scored by several workgroups that leave the
+// keys in memory (vk_page_scores) for a second launch (vk_page_topk).
+constexpr int kSelThreads = 64 * kSelWaves;
 
+// What a workgroup of the selection knows of its (sequence, KV head).
+struct SelUnit {
+  int s, kvh, np, lo, n;   // pages of the context; the scored ones are [lo, lo + n)
+  const int32_t* bt;
+};
+DEV SelUnit sel_unit(const SelectParams& P, int unit) {
+  SelUnit u;
+  u.kvh = unit % P.n_kv_heads;
+  u.s = unit / P.n_kv_heads;
+  const int ctx = max(0, min(P.context_lens[u.s], P.cap_tokens));
+  u.np = (ctx + P.page_tokens - 1) / P.page_tokens;
+  u.lo = P.n_first;
+  u.n = u.np > P.n_list ? u.np - P.n_first - P.n_last : 0;  // none: all pages are listed
+  u.bt = P.block_tables + (int64_t)table_row(P.seq_rows, u.s, P.bt_rows) * P.bt_stride;
+  return u;
+}
 
-// Rows of the (sequence, KV head)'s queries as codes in LDS, negative parts first;
-// rows past the group hold zeros. Returns after a barrier.
+// Codes of the (sequence, KV head)'s queries in LDS, negative parts first; rows past
+// the group repeat its last one (their scores change no maximum). Ends with a barrier.
 template <int QT, int T, int RT>
-DEV void load_query_codes(const SelectParams& P, int s, int kvh, int8_t (*qc)[2 * T], float* qs) {
+DEV void load_query_codes(const SelectParams& P, const SelUnit& u, int8_t (*qc)[2 * T], float* qs) {
   const int lane = lane_id(), w = (int)threadIdx.x / WAVE, G = P.n_heads / P.n_kv_heads;
   constexpr int EPL = T / WAVE;
   for (int r = w; r < 16 * RT; r += kSelWaves) {
     float x[EPL], bad = 0.0f, top = 0.0f;
-    const int64_t row = ((int64_t)s * P.n_heads + (int64_t)kvh * G + min(r, G - 1)) * P.io_hd;
+    const int64_t row = ((int64_t)u.s * P.n_heads + (int64_t)u.kvh * G + min(r, G - 1)) * P.io_hd;
 #pragma unroll
     for (int e = 0; e < EPL; ++e) {
       const int d = lane * EPL + e;
-      x[e] = 0.0f;
-      if (r < G && d < P.io_hd)
-        x[e] = QT == DT_F32 ? reinterpret_cast<const float*>(P.q)[row + d] : h2f(reinterpret_cast<const uint16_t*>(P.q)[row + d]);
+      const int64_t at = row + min(d, P.io_hd - 1);
+      x[e] = QT == DT_F32 ? reinterpret_cast<const float*>(P.q)[at] : h2f(reinterpret_cast<const uint16_t*>(P.q)[at]);
+      x[e] = d < P.io_hd ? x[e] : 0.0f;
       top = fmaxf(top, fabsf(x[e]));
       bad = fmaf(x[e], 0.0f, bad);
     }
@@ -204,20 +335,47 @@ DEV void load_query_codes(const SelectParams& P, int s, int kvh, int8_t (*qc)[2 
   __syncthreads();
 }
 
+// A wave's turn of 64 scored pages: their ids, codes and scales. keys[i] is page u.lo + i.
+template <int T>
+struct PageTurn {
+  static constexpr int KJ = 2 * T / 64;  // products of 64 dims
+  int raw;          // the lane's page id
+  i32x4 kb[4][KJ];  // codes of page 16 v + n, as operands
+  float scale;
+};
+DEV int page_id(const SelectParams& P, const SelUnit& u, int p) { return u.bt[u.lo + min(p + lane_id(), u.n - 1)]; }
+template <int T>
+DEV void load_turn(const SelectParams& P, const SelUnit& u, int raw, PageTurn<T>& t) {
+  const int lane = lane_id(), n = lane & 15, g = lane >> 4;
+  const int page = min(max(raw, 0), P.n_pool_pages - 1);
+  t.raw = raw;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    const int64_t at = (int64_t)__shfl(page, 16 * v + n, WAVE) * P.n_kv_heads + u.kvh;
+    const i32x4* c = reinterpret_cast<const i32x4*>(P.codes + at * 2 * T + 16 * g);
+#pragma unroll
+    for (int j = 0; j < PageTurn<T>::KJ; ++j) t.kb[v][j] = c[4 * j];
+  }
+  t.scale = P.scales[(int64_t)page * P.n_kv_heads + u.kvh];
+}
+
+// Keys of scored pages first, first + step, ..: 64 a turn, as four products of 16 pages
+// (the pages are the columns, the heads the rows). The first turn's loads are issued
+// before the queries' codes are made. Returns the lane's least and largest key.
 template <int QT, int T, int RT>
-DEV void page_scores(const SelectParams& P) {
-  constexpr int KJ = 2 * T / 64;  // products of 64 dims
-  __shared__ __align__(16) int8_t qc[16 * RT][2 * T];
-  __shared__ float qs[16 * RT];
-  const int lane = lane_id(), n = lane & 15, g = lane >> 4, w = (int)threadIdx.x / WAVE;
-  const int chunk = (int)(blockIdx.x % P.n_chunks);
-  const int unit = (int)(blockIdx.x / P.n_chunks);
-  const int kvh = unit % P.n_kv_heads, s = unit / P.n_kv_heads;
-  const int G = P.n_heads / P.n_kv_heads;
-  const int ctx = max(0, min(P.context_lens[s], P.cap_tokens));
-  const int np = (ctx + P.page_tokens - 1) / P.page_tokens;
-  if (np <= P.n_list) return;  // all pages are listed
-  load_query_codes<QT, T, RT>(P, s, kvh, qc, qs);
+DEV uint2 score_pages(const SelectParams& P, const SelUnit& u, int8_t (*qc)[2 * T], float* qs, int first, int step, uint32_t* keys) {
+  constexpr int KJ = PageTurn<T>::KJ;
+  const int lane = lane_id(), n = lane & 15, g = lane >> 4;
+  uint2 span = make_uint2(0xFFFFFFFFu, 0u);
+  PageTurn<T> t;
+  int next = 0;
+  if (first < u.n) {
+    const int raw = page_id(P, u, first);
+    next = page_id(P, u, first + step);
+    load_turn<T>(P, u, raw, t);
+  }
+  load_query_codes<QT, T, RT>(P, u, qc, qs);
+  if (first >= u.n) return span;
   i32x4 qa[RT][KJ];
   float qsc[RT][4];
 #pragma unroll
@@ -227,84 +385,114 @@ DEV void page_scores(const SelectParams& P) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) qsc[rt][i] = qs[16 * rt + 4 * g + i];
   }
-  const int32_t* bt = P.block_tables + (int64_t)table_row(P.seq_rows, s, P.bt_rows) * P.bt_stride;
-  uint32_t* keys = P.keys + (int64_t)unit * P.max_pages;
   bool out = false;
-  for (int p0 = (chunk * kSelWaves + w) * 16; p0 < np; p0 += P.n_chunks * kSelWaves * 16) {
-    const int raw = bt[min(p0 + n, np - 1)];
-    out |= raw < 0 || raw >= P.n_pool_pages;
-    const int64_t at = (int64_t)min(max(raw, 0), P.n_pool_pages - 1) * P.n_kv_heads + kvh;
-    const i32x4* c = reinterpret_cast<const i32x4*>(P.codes + at * 2 * T + 16 * g);
-    i32x4 kb[KJ];
+  for (int p0 = first; p0 < u.n; p0 += step) {
+    out |= t.raw < 0 || t.raw >= P.n_pool_pages;
+    float best[4];
 #pragma unroll
-    for (int j = 0; j < KJ; ++j) kb[j] = c[4 * j];
-    const float scale = P.scales[at];
-    float best = -kInf;  // a score that is not a number counts as this
+    for (int v = 0; v < 4; ++v) {
+      const float sc = __shfl(t.scale, 16 * v + n, WAVE);
+      best[v] = -kInf;  // a score that is not a number counts as this
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      i32x4 dot = {0, 0, 0, 0};
+      for (int rt = 0; rt < RT; ++rt) {
+        i32x4 dot = {0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < KJ; ++j) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[rt][j], kb[j], dot, 0, 0, 0);
+        for (int j = 0; j < KJ; ++j) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[rt][j], t.kb[v][j], dot, 0, 0, 0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = ((float)dot[i] * scale) * qsc[rt][i];
-        if (16 * rt + 4 * g + i < G) best = fmaxf(best, x);
+        for (int i = 0; i < 4; ++i) best[v] = fmaxf(best[v], ((float)dot[i] * sc) * qsc[rt][i]);
       }
     }
-    best = fmaxf(best, shfl_xor(best, 16));
-    best = fmaxf(best, shfl_xor(best, 32));
-    const int page = p0 + n;
-    uint32_t key = order_key(scale == kInf ? kInf : best);
-    if (page < P.n_first || page >= np - P.n_last) key = kKeyKept;
-    if (g == 0 && page < np) keys[page] = key;
+    const bool top = t.scale == kInf;
+    if (p0 + step < u.n) {
+      const int raw = next;
+      next = page_id(P, u, p0 + 2 * step);
+      load_turn<T>(P, u, raw, t);
+    }
+    // the maximum over the row groups, which leaves lane l page p0 + l's
+    swap_lanes<32>(best[0], best[2]);
+    swap_lanes<32>(best[1], best[3]);
+    float a = fmaxf(best[0], best[2]), b = fmaxf(best[1], best[3]);
+    swap_lanes<16>(a, b);
+    const uint32_t key = order_key(top ? kInf : fmaxf(a, b));
+    if (p0 + lane < u.n) {
+      keys[p0 + lane] = key;
+      span.x = min(span.x, key);
+      span.y = max(span.y, key);
+    }
   }
   if (__builtin_amdgcn_ballot_w64(out) != 0 && lane == 0) flag_misuse(P.err, MISUSE_PAGE_OUT_OF_POOL);
+  return span;
 }
 
-// The n_list pages with the largest keys, ties to the lower page, in ascending order.
-// Radix selection: each round counts the next 8 bits of the keys that share the bits
-// found so far and keeps the bin that holds the n_list-th largest; the last round
-// leaves that key and how many of its equals belong to the list.
-DEV void page_topk(const SelectParams& P) {
-  __shared__ int hist[256];
-  __shared__ int found[2];  // bin, keys still wanted in it
-  __shared__ int wsum[2][kSelWaves];
+DEV uint32_t wave_max_u(uint32_t x) {
+  x = max(x, dpp_u<DPP_QUAD_XOR1>(x, x));
+  x = max(x, dpp_u<DPP_QUAD_XOR2>(x, x));
+  x = max(x, dpp_u<DPP_ROW_HALF_MIRROR>(x, x));
+  x = max(x, dpp_u<DPP_ROW_MIRROR>(x, x));
+  return max(max((uint32_t)readlane_i((int)x, 0), (uint32_t)readlane_i((int)x, 16)),
+             max((uint32_t)readlane_i((int)x, 32), (uint32_t)readlane_i((int)x, 48)));
+}
+// Sum over lanes 0 .. l.
+DEV int wave_prefix_sum(int x) {
+  x += (int)dpp_u<0x111>((uint32_t)x, 0);  // row_shr 1, 2, 4, 8
+  x += (int)dpp_u<0x112>((uint32_t)x, 0);
+  x += (int)dpp_u<0x114>((uint32_t)x, 0);
+  x += (int)dpp_u<0x118>((uint32_t)x, 0);
+  const int lane = lane_id(), a = readlane_i(x, 15), b = readlane_i(x, 31), c = readlane_i(x, 47);
+  return x + (lane >= 16 ? a : 0) + (lane >= 32 ? b : 0) + (lane >= 48 ? c : 0);
+}
+
+// Writes a (sequence, KV head)'s list: the kept pages and, of the scored ones, the
+// `want` with the largest keys, ties to the lower page, in ascending order. The want-th
+// largest key is found in rounds: the keys in question lie in [base, base + 2^bits);
+// their 8 leading bits are counted, and the bin that holds the key sought is the next
+// round's range. A bin of at most 64 keys is ranked by one wave.
+struct SelScratch {
+  int hist[256];
+  int turn[kSelWaves][2];
+  uint32_t least, most, bin_keys[64];
+  int n_bin, found[3];
+};
+DEV void select_begin(SelScratch& x) {  // before a barrier
+  if (threadIdx.x == 0) { x.least = 0xFFFFFFFFu; x.most = 0; }
+}
+template <typename Keys>
+DEV void select_top(const SelectParams& P, const SelUnit& u, const Keys keys, uint2 span, int32_t* pages, SelScratch& x) {
   const int tid = (int)threadIdx.x, lane = lane_id(), w = tid / WAVE;
-  const int unit = (int)blockIdx.x, s = unit / P.n_kv_heads;
-  const int ctx = max(0, min(P.context_lens[s], P.cap_tokens));
-  const int np = (ctx + P.page_tokens - 1) / P.page_tokens;
-  int32_t* pages = P.pages + (int64_t)unit * P.n_list;
-  if (np <= P.n_list) {
-    for (int i = tid; i < P.n_list; i += 64 * kSelWaves) pages[i] = i < np ? i : -1;
-    return;
-  }
-  const uint32_t* keys = P.keys + (int64_t)unit * P.max_pages;
-  uint32_t prefix = 0;
-  int want = P.n_list;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    hist[tid] = 0;
+  const int want_all = P.n_list - P.n_first - P.n_last;
+  for (int i = tid; i < P.n_first; i += kSelThreads) pages[i] = i;
+  for (int i = tid; i < P.n_last; i += kSelThreads) pages[P.n_list - P.n_last + i] = u.np - P.n_last + i;
+  if (want_all == 0) return;
+  const uint32_t least = ~wave_max_u(~span.x), most = wave_max_u(span.y);
+  if (lane == 0) { atomicMin(&x.least, least); atomicMax(&x.most, most); }
+  __syncthreads();
+  uint32_t base = x.least;
+  const uint32_t range = x.most - base;
+  int bits = range ? 32 - __builtin_clz(range) : 0, want = want_all;
+  uint32_t key = base;  // the want_all-th largest, `want` of whose equals are listed
+  while (bits > 0) {
+    const int shift = max(0, bits - 8);
+    if (tid < 256) x.hist[tid] = 0;
+    if (tid == 0) x.n_bin = 0;
     __syncthreads();
-    for (int i = tid; i < np; i += 64 * kSelWaves) {
-      const uint32_t k = keys[i];
-      if (shift == 24 || k >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&hist[(k >> shift) & 255u], 1);
+    for (int i = tid; i < u.n; i += kSelThreads) {
+      const uint32_t k = keys[i] - base;
+      if (bits == 32 || k >> bits == 0) atomicAdd(&x.hist[k >> shift], 1);
     }
     __syncthreads();
     if (w == 0) {  // bins 255 - 4 l - e of lane l, largest first
       int c[4], sum = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { c[e] = hist[255 - 4 * lane - e]; sum += c[e]; }
-      int incl = sum;
-      for (int m = 1; m < WAVE; m *= 2) {
-        const int up = __shfl_up(incl, m, WAVE);
-        if (lane >= m) incl += up;
-      }
+      for (int e = 0; e < 4; ++e) { c[e] = x.hist[255 - 4 * lane - e]; sum += c[e]; }
+      const int incl = wave_prefix_sum(sum);
       int before = incl - sum;
       if (before < want && incl >= want) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (before < want && before + c[e] >= want) {
-            found[0] = 255 - 4 * lane - e;
-            found[1] = want - before;
+            x.found[0] = 255 - 4 * lane - e;
+            x.found[1] = want - before;
+            x.found[2] = c[e];
             before = want;  // no later bin
           } else {
             before += c[e];
@@ -313,30 +501,110 @@ DEV void page_topk(const SelectParams& P) {
       }
     }
     __syncthreads();
-    prefix |= (uint32_t)found[0] << shift;
-    want = found[1];
-    __syncthreads();
-  }
-  // prefix is the n_list-th largest key: every larger one is listed, and the first `want` equal ones
-  int above = 0, equal = 0;  // before this round's pages
-  for (int p0 = 0; p0 < np; p0 += 64 * kSelWaves) {
-    const int i = p0 + tid;
-    const uint32_t k = i < np ? keys[i] : 0u;
-    const uint64_t gt = __builtin_amdgcn_ballot_w64(i < np && k > prefix), eq = __builtin_amdgcn_ballot_w64(i < np && k == prefix);
-    if (lane == 0) { wsum[0][w] = __builtin_popcountll(gt); wsum[1][w] = __builtin_popcountll(eq); }
-    __syncthreads();
-    int a = above, e = equal;
-    for (int v = 0; v < kSelWaves; ++v) {
-      if (v < w) { a += wsum[0][v]; e += wsum[1][v]; }
-      above += wsum[0][v];
-      equal += wsum[1][v];
+    base += (uint32_t)x.found[0] << shift;
+    want = x.found[1];
+    key = base;
+    bits = shift;
+    const int m = x.found[2];
+    if (bits == 0) break;  // the bin is one key
+    if (m > WAVE) { __syncthreads(); continue; }
+    // the m keys of the bin: the want-th largest
+    for (int i = tid; i < u.n; i += kSelThreads) {
+      const uint32_t k = keys[i];
+      if ((k - base) >> bits == 0) x.bin_keys[atomicAdd(&x.n_bin, 1)] = k;
     }
-    const uint64_t below = (1ull << lane) - 1;
-    a += __builtin_popcountll(gt & below);
-    e += __builtin_popcountll(eq & below);
-    if (i < np && (k > prefix || (k == prefix && e < want))) pages[a + min(e, want)] = i;
     __syncthreads();
+    const uint32_t mine = x.bin_keys[lane];
+    int above = 0, equal = 0;
+    for (int j = 0; j < m; ++j) {
+      const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)mine, j);
+      above += o > mine;
+      equal += o == mine;
+    }
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(lane < m && above < want && above + equal >= want);
+    const int l = __builtin_ctzll(hit);
+    key = (uint32_t)__builtin_amdgcn_readlane((int)mine, l);
+    want -= __builtin_amdgcn_readlane(above, l);
+    break;
   }
+  __syncthreads();
+  // a wave's share of the pages is one run of them, so that its place in the list follows
+  // from how many the waves before it list
+  const int per = (u.n + kSelThreads - 1) / kSelThreads * WAVE;
+  const int i0 = w * per, i1 = min(u.n, i0 + per);
+  int above = 0, equal = 0;
+  for (int i = i0 + lane; i - lane < i1; i += WAVE) {
+    const uint32_t k = i < i1 ? keys[i] : 0;
+    above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i < i1 && k > key));
+    equal += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i < i1 && k == key));
+  }
+  if (lane == 0) { x.turn[w][0] = above; x.turn[w][1] = equal; }
+  __syncthreads();
+  above = equal = 0;
+  for (int v = 0; v < w; ++v) { above += x.turn[v][0]; equal += x.turn[v][1]; }
+  pages += P.n_first;
+  for (int i = i0 + lane; i - lane < i1; i += WAVE) {
+    const uint32_t k = i < i1 ? keys[i] : 0;
+    const uint64_t gt = __builtin_amdgcn_ballot_w64(i < i1 && k > key), eq = __builtin_amdgcn_ballot_w64(i < i1 && k == key);
+    const uint64_t below = (1ull << lane) - 1;
+    const int e = equal + __builtin_popcountll(eq & below);
+    if (i < i1 && (k > key || (k == key && e < want))) pages[above + __builtin_popcountll(gt & below) + min(e, want)] = u.lo + i;
+    above += __builtin_popcountll(gt);
+    equal += __builtin_popcountll(eq);
+  }
+}
+
+// A context of no more pages than the list has places: all of them.
+DEV void list_all(const SelectParams& P, const SelUnit& u, int32_t* pages) {
+  for (int i = (int)threadIdx.x; i < P.n_list; i += kSelThreads) pages[i] = i < u.np ? i : -1;
+}
+
+// The wave's first page of a workgroup's chunk.
+DEV int first_page(int chunk) { return chunk * kSelThreads + __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE) * WAVE; }
+
+template <int QT, int T, int RT>
+DEV void page_select(const SelectParams& P) {
+  __shared__ __align__(16) int8_t qc[16 * RT][2 * T];
+  __shared__ float qs[16 * RT];
+  __shared__ uint32_t keys[kSelPages];
+  __shared__ SelScratch scratch;
+  const SelUnit u = sel_unit(P, (int)blockIdx.x);
+  int32_t* pages = P.pages + (int64_t)blockIdx.x * P.n_list;
+  if (u.n == 0) {
+    list_all(P, u, pages);
+    return;
+  }
+  select_begin(scratch);
+  const uint2 span = score_pages<QT, T, RT>(P, u, qc, qs, first_page(0), kSelThreads, keys);
+  select_top(P, u, keys, span, pages, scratch);
+}
+
+template <int QT, int T, int RT>
+DEV void page_scores(const SelectParams& P) {
+  __shared__ __align__(16) int8_t qc[16 * RT][2 * T];
+  __shared__ float qs[16 * RT];
+  const int chunk = (int)(blockIdx.x % P.n_chunks), unit = (int)(blockIdx.x / P.n_chunks);
+  const SelUnit u = sel_unit(P, unit);
+  if (chunk * kSelThreads >= u.n) return;
+  score_pages<QT, T, RT>(P, u, qc, qs, first_page(chunk), P.n_chunks * kSelThreads, P.keys + (int64_t)unit * P.max_pages);
+}
+DEV void page_topk(const SelectParams& P) {
+  __shared__ SelScratch scratch;
+  const SelUnit u = sel_unit(P, (int)blockIdx.x);
+  int32_t* pages = P.pages + (int64_t)blockIdx.x * P.n_list;
+  if (u.n == 0) {
+    list_all(P, u, pages);
+    return;
+  }
+  const uint32_t* keys = P.keys + (int64_t)blockIdx.x * P.max_pages;
+  select_begin(scratch);
+  uint2 span = make_uint2(0xFFFFFFFFu, 0u);
+  for (int i = (int)threadIdx.x; i < u.n; i += kSelThreads) {
+    const uint32_t k = keys[i];
+    span = make_uint2(min(span.x, k), max(span.y, k));
+  }
+  __syncthreads();
+  select_top(P, u, keys, span, pages, scratch);
 }
 
 // =============================================================================
@@ -467,6 +735,15 @@ DEV int sparse_qdim(int j, int g) {
   else return 32 * j + 8 * g;
 }
 
+// N query values, wherever they start.
+template <int QT, int N>
+DEV void load_q(const void* q, int64_t at, float (&x)[N]) {
+  typedef uint32_t words __attribute__((ext_vector_type(QT == DT_F32 ? N : N / 2), aligned(2)));
+  const words r = *reinterpret_cast<const words*>(reinterpret_cast<const uint8_t*>(q) + at * (QT == DT_F32 ? 4 : 2));
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = QT == DT_F32 ? bitcast<float>(r[i]) : i % 2 ? half_hi(r[i / 2]) : half_lo(r[i / 2]);
+}
+
 template <int KV, int QT, int T, int RT>
 DEV void sparse_attn(const SparseParams& P) {
   constexpr bool F32 = KV == KV_F32, BLK = KV == KV_I8_BLK, REF = KV == KV_I8_REF;
@@ -486,6 +763,38 @@ DEV void sparse_attn(const SparseParams& P) {
   const int G = P.n_heads / P.n_kv_heads;
   const int ctx = max(0, min(P.context_lens[s], P.cap_tokens));
   const int64_t row0 = (int64_t)s * P.n_heads + (int64_t)kvh * G;
+
+  // q^T: row n of each 16-row tile (rows past the group repeat its last one: their columns of
+  // the results are not used), zeros past head_dim
+  half8 qa[RT][F32 ? 1 : KC], qlo[RT][QSPLIT ? KC : 1];
+  float qf[RT][F32 ? T / 4 : 1];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int64_t off = (row0 + min(16 * rt + n, G - 1)) * P.io_hd;
+    if constexpr (F32) {
+#pragma unroll
+      for (int j = 0; j < T / 16; ++j) {
+        const int d = 16 * j + 4 * g;
+        float x[4];
+        load_q<QT, 4>(P.q, off + min(d, P.io_hd - 4), x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qf[rt][4 * j + e] = d < P.io_hd ? x[e] : 0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < KC; ++j) {
+        const int d = sparse_qdim<KV, T>(j, g);
+        float x[8];
+        load_q<QT, 8>(P.q, off + min(d, P.io_hd - 8), x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float v = d < P.io_hd ? x[i] : 0.0f;
+          qa[rt][j][i] = (_Float16)v;
+          if constexpr (QSPLIT) qlo[rt][j][i] = (_Float16)(v - (float)qa[rt][j][i]);
+        }
+      }
+    }
+  }
 
   if (w == 0) {  // the part's entries that name a page of the context
     const int32_t* bt = P.block_tables + (int64_t)table_row(P.seq_rows, s, P.bt_rows) * P.bt_stride;
@@ -511,48 +820,6 @@ DEV void sparse_attn(const SparseParams& P) {
   }
   __syncthreads();
   const int n_tiles = __builtin_amdgcn_readfirstlane(n_valid) * P.page_tiles;
-
-  // q^T: row n of each 16-row tile, zeros past the group and past head_dim
-  half8 qa[RT][F32 ? 1 : KC], qlo[RT][QSPLIT ? KC : 1];
-  float qf[RT][F32 ? T / 4 : 1];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = 16 * rt + n;
-    const int64_t off = (row0 + min(r, G - 1)) * P.io_hd;
-    if constexpr (F32) {
-#pragma unroll
-      for (int j = 0; j < T / 16; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int d = 16 * j + 4 * g + e;
-          float x = 0.0f;
-          if (r < G && d < P.io_hd)
-            x = QT == DT_F32 ? reinterpret_cast<const float*>(P.q)[off + d] : h2f(reinterpret_cast<const uint16_t*>(P.q)[off + d]);
-          qf[rt][4 * j + e] = x;
-        }
-    } else {
-#pragma unroll
-      for (int j = 0; j < KC; ++j) {
-        const int d = sparse_qdim<KV, T>(j, g);
-        half8 x = {0, 0, 0, 0, 0, 0, 0, 0}, lo = x;
-        if (r < G && d < P.io_hd) {
-          if constexpr (QT == DT_F32) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float v = reinterpret_cast<const float*>(P.q)[off + d + i];
-              x[i] = (_Float16)v;
-              lo[i] = (_Float16)(v - (float)x[i]);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = bitcast<_Float16>(reinterpret_cast<const uint16_t*>(P.q)[off + d + i]);
-          }
-        }
-        qa[rt][j] = x;
-        if constexpr (QSPLIT) qlo[rt][j] = lo;
-      }
-    }
-  }
 
   f32x4 acc[RT][NT];
   float M[RT], L[RT];
@@ -693,23 +960,40 @@ DEV void sparse_attn(const SparseParams& P) {
   }
 }
 
-// Joins the parts of a row: one wave a row, T / 64 dims a lane.
+// Joins the parts of a row: one wave a row, T / 64 dims a lane; lane v holds part v's
+// maximum and sum, 64 parts a turn.
 template <int T>
 DEV void sparse_merge(const SparseParams& P) {
-  constexpr int EPL = T / WAVE;
+  constexpr int EPL = T / WAVE, UN = 8;
   const int lane = lane_id();
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x / WAVE) + threadIdx.x / WAVE;
   if (row >= (int64_t)P.n_seqs * P.n_heads) return;
   const float2* ml = reinterpret_cast<const float2*>(P.part_ml) + row * P.n_splits;
   const float* acc = P.part_acc + row * P.n_splits * T + lane * EPL;
   float m = -kInf, l = 0.0f, o[EPL] = {};
-  for (int v = 0; v < P.n_splits; ++v) m = fmaxf(m, ml[v].x);
-  for (int v = 0; v < P.n_splits; ++v) {
-    const float2 x = ml[v];
-    const float f = x.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(x.x - m);
-    l = fmaf(f, x.y, l);
+  for (int v0 = 0; v0 < P.n_splits; v0 += WAVE) {
+    const int nv = min(WAVE, P.n_splits - v0);
+    const float2 x = ml[v0 + min(lane, nv - 1)];
+    const float xm = lane < nv ? x.x : -kInf, top = fmaxf(m, wave_max(xm));
+    const float f = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - top);  // of the turns before
+    const float part = xm == -kInf ? 0.0f : __builtin_amdgcn_exp2f(xm - top);
+    m = top;
+    l = l * f + wave_sum(part * x.y);
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) o[e] = fmaf(f, acc[(int64_t)v * T + e], o[e]);
+    for (int e = 0; e < EPL; ++e) o[e] *= f;
+    for (int v = 0; v < nv; v += UN) {
+      float a[UN][EPL];
+#pragma unroll
+      for (int i = 0; i < UN; ++i)
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) a[i][e] = acc[(int64_t)(v0 + min(v + i, nv - 1)) * T + e];
+#pragma unroll
+      for (int i = 0; i < UN; ++i) {
+        const float s = v + i < nv ? readlane_f(part, v + i) : 0.0f;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) o[e] = fmaf(s, a[i][e], o[e]);
+      }
+    }
   }
 #pragma unroll
   for (int e = 0; e < EPL; ++e)
@@ -722,18 +1006,17 @@ DEV void sparse_merge(const SparseParams& P) {
   extern "C" __global__ void __launch_bounds__(THREADS) NAME(const PARAMS P) { BODY; }
 
 #define VK_INDEX(KV)                                                                   \
-  VK_KERNEL(vk_index_update_kv##KV, 256, IndexUpdateParams, (index_update<KV, 128>(P)))  \
-  VK_KERNEL(vk_index_update_kv##KV##_d64, 256, IndexUpdateParams, (index_update<KV, 64>(P)))
+  VK_KERNEL(vk_index_update_kv##KV, kUpdateThreads, IndexUpdateParams, (index_update<KV, 128>(P)))  \
+  VK_KERNEL(vk_index_update_kv##KV##_d64, kUpdateThreads, IndexUpdateParams, (index_update<KV, 64>(P)))
 VK_INDEX(0) VK_INDEX(1) VK_INDEX(2) VK_INDEX(3)
 VK_KERNEL(vk_index_read, 256, IndexReadParams, index_read(P))
 
-#define VK_SCORES(QT)                                                                              \
-  VK_KERNEL(vk_page_scores_r1_q##QT, 64 * kSelWaves, SelectParams, (page_scores<QT, 128, 1>(P)))      \
-  VK_KERNEL(vk_page_scores_r2_q##QT, 64 * kSelWaves, SelectParams, (page_scores<QT, 128, 2>(P)))      \
-  VK_KERNEL(vk_page_scores_d64_r1_q##QT, 64 * kSelWaves, SelectParams, (page_scores<QT, 64, 1>(P)))   \
-  VK_KERNEL(vk_page_scores_d64_r2_q##QT, 64 * kSelWaves, SelectParams, (page_scores<QT, 64, 2>(P)))
-VK_SCORES(0) VK_SCORES(1)
-VK_KERNEL(vk_page_topk, 64 * kSelWaves, SelectParams, page_topk(P))
+#define VK_SELECT(TAG, QT, T, RT)                                                             \
+  VK_KERNEL(vk_page_select##TAG, kSelThreads, SelectParams, (page_select<QT, T, RT>(P)))       \
+  VK_KERNEL(vk_page_scores##TAG, kSelThreads, SelectParams, (page_scores<QT, T, RT>(P)))
+VK_SELECT(_r1_q0, 0, 128, 1) VK_SELECT(_r2_q0, 0, 128, 2) VK_SELECT(_d64_r1_q0, 0, 64, 1) VK_SELECT(_d64_r2_q0, 0, 64, 2)
+VK_SELECT(_r1_q1, 1, 128, 1) VK_SELECT(_r2_q1, 1, 128, 2) VK_SELECT(_d64_r1_q1, 1, 64, 1) VK_SELECT(_d64_r2_q1, 1, 64, 2)
+VK_KERNEL(vk_page_topk, kSelThreads, SelectParams, page_topk(P))
 
 #define VK_SPARSE(KV, QT)                                                                                          \
   VK_KERNEL(vk_sparse_kv##KV##_r1_q##QT, 64 * kSparseMaxWaves, SparseParams, (sparse_attn<KV, QT, 128, 1>(P)))         \
