@@ -12,6 +12,7 @@ constexpr int32_t kMaxVocab = 1 << 28;
 
 struct LogprobPlan {
   int parts, part_len;
+  bool whole;  // a row is one workgroup of 16 waves
   uint64_t sums_bytes, top_bytes;
 };
 
@@ -25,11 +26,13 @@ int plan_logprobs(const vk_ctx* ctx, const vk_logprob_args* a, LogprobPlan* pl) 
   if (a->n_top > kMaxTop) return fail(VK_ERR_UNSUPPORTED, "n_top %d (up to %d)", a->n_top, kMaxTop);
   if (a->n_top > a->vocab) return fail(VK_ERR_BAD_ARG, "n_top %d exceeds the vocabulary (%d)", a->n_top, a->vocab);
   if (!(a->scale >= 0.f) || std::isinf(a->scale)) return fail(VK_ERR_BAD_ARG, "scale must be finite and not negative");
-  // parts of 8192 values (a step of a workgroup) at least, about four workgroups a CU
+  // Parts of 8192 values (a step of a workgroup of four waves) at least, about four
+  // workgroups a CU; a few short rows take one workgroup of 16 waves each, and no join.
   constexpr int kStep = 8192;
   const int64_t rows = std::max<int64_t>(1, a->n_rows);
   const int64_t steps = ((int64_t)a->vocab + kStep - 1) / kStep;
-  const int64_t want = std::max<int64_t>(1, std::min({(4 * ctx->n_cu + rows - 1) / rows, steps, (int64_t)kMaxLogitParts}));
+  pl->whole = rows <= ctx->n_cu && steps > 1 && steps <= 4;
+  const int64_t want = pl->whole ? 1 : std::max<int64_t>(1, std::min({(4 * ctx->n_cu + rows - 1) / rows, steps, (int64_t)kMaxLogitParts}));
   const int64_t per = (steps + want - 1) / want;
   pl->part_len = (int)std::min<int64_t>(per * kStep, kMaxVocab);
   pl->parts = (int)((steps + per - 1) / per);
@@ -38,14 +41,14 @@ int plan_logprobs(const vk_ctx* ctx, const vk_logprob_args* a, LogprobPlan* pl) 
     pl->sums_bytes = align_up((uint64_t)a->n_rows * pl->parts * 4 * sizeof(float), 256);
     pl->top_bytes = align_up((uint64_t)a->n_rows * pl->parts * a->n_top * sizeof(uint64_t), 256);
   }
-  if ((uint64_t)a->n_rows * pl->parts * 256 >= 1ull << 32) return fail(VK_ERR_UNSUPPORTED, "grid too large");
+  if ((uint64_t)a->n_rows * pl->parts * (pl->whole ? 1024 : 256) >= 1ull << 32) return fail(VK_ERR_UNSUPPORTED, "grid too large");
   return VK_OK;
 }
 
 }  // namespace
 
 std::vector<std::string> velokv::logits_kernel_names() {
-  return {"vk_logprob_part_q0", "vk_logprob_part_q1", "vk_logprob_join_q0", "vk_logprob_join_q1"};
+  return {"vk_logprob_part_q0", "vk_logprob_part_q1", "vk_logprob_row_q0", "vk_logprob_row_q1", "vk_logprob_join_q0", "vk_logprob_join_q1"};
 }
 
 extern "C" int vk_token_logprobs_workspace(const vk_ctx* ctx, const vk_logprob_args* a, uint64_t* bytes) {
@@ -92,6 +95,7 @@ extern "C" int vk_token_logprobs(vk_ctx* ctx, const vk_logprob_args* a, void* st
   p.part_len = pl.part_len;
   p.scale = a->scale != 0.f ? a->scale : 1.f;
   const std::string dt = std::to_string(a->dtype);
+  if (pl.whole) return launch(ctx, ("vk_logprob_row_q" + dt).c_str(), dim3((unsigned)a->n_rows), dim3(1024), p, stream);
   rc = launch(ctx, ("vk_logprob_part_q" + dt).c_str(), dim3((unsigned)((uint64_t)a->n_rows * pl.parts)), dim3(256), p, stream);
   if (rc || pl.parts == 1) return rc;
   return launch(ctx, ("vk_logprob_join_q" + dt).c_str(), dim3((unsigned)a->n_rows), dim3(256), p, stream);

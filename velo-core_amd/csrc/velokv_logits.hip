@@ -13,35 +13,32 @@ constexpr int kList = 512;       // candidates of a wave
 constexpr int kStepValues = 32;  // values of a thread in a step
 
 // =============================================================================
-// Log probabilities of a row x (logits times scale): with M = max x,
-//     Z = sum e^(x - M),  T = sum e^(x - M) (x - M),
-//     log p_t = (x_t - M) - log Z,   entropy = log Z - T / Z,
+// Log probabilities of a row of logits x, in units of log 2: with c = scale log2(e) and
+// m = max x,
+//     e_v = (x_v - m) c,  Z = sum 2^e_v,  T = sum 2^e_v e_v,
+//     log p_t = (x_t - m) scale - log2 Z ln 2,   entropy = (log2 Z - T / Z) ln 2,
 // and the n_top largest x, ties to the lower index. One pass over the row: every
-// thread keeps its own running M, Z and T; a wave keeps a list of candidates for the
-// largest values. A candidate is one 64-bit word, the value as an ordered key above
-// the complement of its index, so that words differ and their order is the order
-// wanted. In the first step a workgroup takes the n_top-th largest of the maxima of 32
-// groups of its lanes: at least n_top values reach it, and few more. Only those, and
-// later values above it, are candidates. A wave whose list they do not fit (equal or
-// rising values) works vector by vector with words of its own as the bound.
+// thread keeps its own m, Z and T; a wave keeps a list of candidates for the largest
+// values. A candidate is one 64-bit word, the value as an ordered key above the
+// complement of its index, so that words differ and their order is the order wanted. In
+// the first step a workgroup takes
+// the n_top-th largest of the maxima of 32 groups of its lanes: at least n_top values
+// reach it, and few more. Only those, and later values above it, are candidates. A wave
+// whose list they do not fit (equal or rising values) works vector by vector with words
+// of its own as the bound.
 // =============================================================================
 struct Sums { float m, z, t; };
 
-// a and b joined; c = scale * log2(e).
-DEV Sums join(const Sums& a, const Sums& b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -kInf) return Sums{m, a.z + b.z, a.t + b.t};  // sums are 0, or NaN
-  const float fa = __builtin_amdgcn_exp2f((a.m - m) * c), fb = __builtin_amdgcn_exp2f((b.m - m) * c);
-  Sums r{m, fa * a.z + fb * b.z, 0.0f};
-  // (a factor of 0 stands beside sums whose product with the distance may overflow)
-  if (fa != 0.0f) r.t += fa * (a.t + a.z * (a.m - m));
-  if (fb != 0.0f) r.t += fb * (b.t + b.z * (b.m - m));
-  return r;
+// Sums taken from their maximum to the larger one m.
+DEV Sums refer(const Sums& s, float m, float c) {
+  const float e = s.m == m ? 0.0f : (s.m - m) * c, f = __builtin_amdgcn_exp2f(e);
+  // (a factor of 0 may stand beside a product that is not finite)
+  return Sums{m, f * s.z, f == 0.0f ? 0.0f : f * fmaf(s.z, e, s.t)};
 }
-DEV Sums wave_join(Sums a, float c) {
-#pragma unroll
-  for (int m = 1; m < WAVE; m *= 2) a = join(a, Sums{shfl_xor(a.m, m), shfl_xor(a.z, m), shfl_xor(a.t, m)}, c);
-  return a;
+// The wave's sums, in every lane.
+DEV Sums wave_join(const Sums& s, float c) {
+  const Sums a = refer(s, wave_max(s.m), c);
+  return Sums{a.m, wave_sum(a.z), wave_sum(a.t)};
 }
 
 DEV uint64_t word_of(float x, int index) {
@@ -92,23 +89,30 @@ DEV int trim_list(uint64_t* list, int n, int k) {
   return push_words(list, 0, x, least);
 }
 
-// The row's results from its sums and its k largest words, sorted.
 template <int DT>
-DEV void write_row(const LogprobParams& P, int row, const Sums& s, const uint64_t* top) {
-  const float log_z = logf(s.z);
-  const auto logprob = [&](float x) { return s.m == -kInf && s.z == 0.0f ? -kInf : (x - s.m) * P.scale - log_z; };
+DEV float logit(const LogprobParams& P, int row, int t) {
+  const int64_t e = (int64_t)row * P.row_stride + t;
+  return DT == DT_F32 ? reinterpret_cast<const float*>(P.logits)[e] : h2f(reinterpret_cast<const uint16_t*>(P.logits)[e]);
+}
+// The logit of given token i of a row; -infinity outside the vocabulary.
+template <int DT>
+DEV float token_logit(const LogprobParams& P, int row, int i) {
+  const int t = P.tokens[(int64_t)row * P.n_tokens + i];
+  return t >= 0 && t < P.vocab ? logit<DT>(P, row, t) : -kInf;
+}
+
+// The row's results from its sums and its k largest words, sorted; x0: the logit of the
+// thread's first token.
+template <int DT>
+DEV void write_row(const LogprobParams& P, int row, const Sums& s, const uint64_t* top, float x0) {
+  constexpr float kLn2 = 0.6931471805599453f;
+  const bool none = s.m == -kInf && s.z == 0.0f;  // every logit is -infinity
+  const float log_z = __builtin_log2f(s.z);
+  const auto logprob = [&](float x) { return none ? -kInf : (x - s.m) * P.scale - log_z * kLn2; };
   const int tid = (int)threadIdx.x;
-  for (int i = tid; i < P.n_tokens; i += (int)blockDim.x) {
-    const int64_t at = (int64_t)row * P.n_tokens + i;
-    const int t = P.tokens[at];
-    float x = -kInf;
-    if (t >= 0 && t < P.vocab) {
-      const int64_t e = (int64_t)row * P.row_stride + t;
-      x = DT == DT_F32 ? reinterpret_cast<const float*>(P.logits)[e] : h2f(reinterpret_cast<const uint16_t*>(P.logits)[e]);
-    }
-    P.token_logprobs[at] = logprob(x);
-  }
-  if (tid == 0 && P.entropy) P.entropy[row] = s.m == -kInf && s.z == 0.0f ? 0.0f : log_z - s.t / s.z * P.scale;
+  for (int i = tid; i < P.n_tokens; i += (int)blockDim.x)
+    P.token_logprobs[(int64_t)row * P.n_tokens + i] = logprob(i == tid ? x0 : token_logit<DT>(P, row, i));
+  if (tid == 0 && P.entropy) P.entropy[row] = none ? 0.0f : (log_z - s.t / s.z) * kLn2;
   if (tid < P.n_top) {
     const int64_t at = (int64_t)row * P.n_top + tid;
     P.top_ids[at] = word_index(top[tid]);
@@ -128,12 +132,12 @@ DEV void rank_words(const uint64_t* words, int n, int k, uint64_t* top) {
 }
 
 // One workgroup of W waves per (row, part). DT: the logits' type.
-template <int DT>
+template <int DT, int W>
 DEV void logprob_part(const LogprobParams& P) {
   constexpr int ESZ = DT == DT_F32 ? 4 : 2;
   constexpr int EPV = 16 / ESZ;             // values of a 16-byte vector
   constexpr int NV = kStepValues / EPV;     // vectors of a thread in a step
-  constexpr int W = kLogitWaves, THREADS = W * WAVE;
+  constexpr int THREADS = W * WAVE;
   constexpr int GROUPS = 32 / W;            // groups of a wave's lanes
   __shared__ uint64_t lists[W][kList];
   __shared__ uint64_t words[W * kMaxTop];
@@ -172,6 +176,7 @@ DEV void logprob_part(const LogprobParams& P) {
     return DT == DT_F32 ? bitcast<float>(r[e]) : e % 2 ? half_hi(r[e / 2]) : half_lo(r[e / 2]);
   };
 
+  const float x0 = P.n_parts == 1 && tid < P.n_tokens ? token_logit<DT>(P, row, tid) : -kInf;
   Sums s{-kInf, 0.0f, 0.0f};
   uint64_t thr = 0;      // candidates of later steps are larger words; 0: not known
   float thr_x = -kInf;   // its value
@@ -201,60 +206,77 @@ DEV void logprob_part(const LogprobParams& P) {
         for (int j = 0; j < 4; ++j) r[i][j] = in ? r[i][j] : DT == DT_F32 ? 0xFF800000u : 0xFC00FC00u;
       }
     }
-    float mv = -kInf;
+    float x[NV][EPV], vm[NV], mv = -kInf;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
 #pragma unroll
-      for (int e = 0; e < EPV; ++e) mv = fmaxf(mv, value(r[i], e));
+      for (int e = 0; e < EPV; ++e) x[i][e] = value(r[i], e);
+      vm[i] = fmaxf(x[i][0], x[i][1]);
+#pragma unroll
+      for (int e = 2; e < EPV; ++e) vm[i] = fmaxf(vm[i], x[i][e]);
+      mv = fmaxf(mv, vm[i]);
+    }
     const float m = first ? fmaxf(mv, x_extra) : mv;
     if (k > 0) {
       bool all = false;  // whether the wave looks at each vector by itself
       if (first) {
-        // the maxima of groups of 8 lanes, and the k-th of the 32 (the vectors' alone: values
+        // the maxima of 32 groups of lanes (the vectors' alone: values
         // of later steps may come before the row's last ones, which are among the extra)
         float gm = fmaxf(mv, dpp<DPP_QUAD_XOR1>(mv));
         gm = fmaxf(gm, dpp<DPP_QUAD_XOR2>(gm));
         gm = fmaxf(gm, dpp<DPP_ROW_HALF_MIRROR>(gm));
+        if constexpr (GROUPS == 2) {
+          gm = fmaxf(gm, dpp<DPP_ROW_MIRROR>(gm));
+          gm = fmaxf(gm, shfl_xor(gm, 16));
+        }
         if (lane % (WAVE / GROUPS) == 0) group_max[w * GROUPS + lane / (WAVE / GROUPS)] = gm;
         __syncthreads();
         const float mine = group_max[lane & 31];
-        int place = 0;
+        if (k > 1) {  // the largest that k of them reach
+          int reach = 0;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float o = readlane_f(mine, j);
-          place += o > mine || (o == mine && j < lane);
+          for (int j = 0; j < 32; ++j) reach += readlane_f(mine, j) >= mine;
+          thr_x = wave_max(reach >= k ? mine : -kInf);
+        } else {
+          thr_x = wave_max(mine);
         }
-        const uint64_t hit = __builtin_amdgcn_ballot_w64(lane < 32 && place == k - 1);
-        thr_x = readlane_f(mine, __builtin_ctzll(hit));
       }
       // candidates: at least thr_x in the first step, above it later
       const bool any = first ? m >= thr_x : m > thr_x;
       if (first && thr_x == -kInf) {
         all = true;
       } else if (__builtin_amdgcn_ballot_w64(any) != 0) {
-        int count = 0;
+        // what the list may have to take, by vectors; where that is too much, counted
+        uint64_t hit[NV];
+        int count = first ? 2 * EPV : 0;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+          hit[i] = __builtin_amdgcn_ballot_w64(first ? vm[i] >= thr_x : vm[i] > thr_x);
+          count += EPV * __builtin_popcountll(hit[i]);
+        }
+        if (n + count > kList) {
+          count = first ? 2 * EPV : 0;
 #pragma unroll
-          for (int e = 0; e < EPV; ++e) {
-            const float x = value(r[i], e);
-            count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(first ? x >= thr_x : x > thr_x));
-          }
-        if (first) count += 2 * EPV;
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < EPV; ++e)
+              count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(first ? x[i][e] >= thr_x : x[i][e] > thr_x));
+        }
         all = n + count > kList;
         if (!all) {
           const uint64_t below = (1ull << lane) - 1;
 #pragma unroll
-          for (int i = 0; i < NV; ++i)
+          for (int i = 0; i < NV; ++i) {
+            if (hit[i] == 0) continue;
 #pragma unroll
             for (int e = 0; e < EPV; ++e) {
-              const float x = value(r[i], e);
-              const bool in = first ? x >= thr_x : x > thr_x;
+              const bool in = first ? x[i][e] >= thr_x : x[i][e] > thr_x;
               const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
               if (mask == 0) continue;
-              if (in) list[n + __builtin_popcountll(mask & below)] = word_of(x, (v0 + i * THREADS + tid) * EPV - off + e);
+              if (in) list[n + __builtin_popcountll(mask & below)] = word_of(x[i][e], (v0 + i * THREADS + tid) * EPV - off + e);
               n += __builtin_popcountll(mask);
             }
+          }
           if (first) {
             const bool in = has_extra && x_extra >= thr_x;
             const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
@@ -272,13 +294,11 @@ DEV void logprob_part(const LogprobParams& P) {
         }
 #pragma unroll 1
         for (int i = 0; i < NV; ++i) {
-          float vm = -kInf;
           u32x4 rv = r[0];
+          float most = vm[0];
 #pragma unroll
-          for (int j = 1; j < NV; ++j) rv = i == j ? r[j] : rv;
-#pragma unroll
-          for (int e = 0; e < EPV; ++e) vm = fmaxf(vm, value(rv, e));
-          if (__builtin_amdgcn_ballot_w64(thr == 0 || vm > thr_x) != 0) {
+          for (int j = 1; j < NV; ++j) { rv = i == j ? r[j] : rv; most = i == j ? vm[j] : most; }
+          if (__builtin_amdgcn_ballot_w64(thr == 0 || most > thr_x) != 0) {
             uint64_t word[EPV];
             const int v = v0 + i * THREADS + tid;
 #pragma unroll
@@ -290,25 +310,20 @@ DEV void logprob_part(const LogprobParams& P) {
         thr = (uint64_t)(order_key(thr_x) + 1) << 32;  // any larger value, whatever its index
       }
     }
-    if (m > s.m) {
-      const float f = __builtin_amdgcn_exp2f((s.m - m) * c);
-      s.t = f == 0.0f ? 0.0f : f * (s.t + s.z * (s.m - m));
-      s.z *= f;
-      s.m = m;
-    }
-    const float at = s.m == -kInf ? 0.0f : s.m;
+    if (m > s.m) s = refer(s, m, c);
+    const float ref = s.m == -kInf ? 0.0f : s.m;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < EPV; ++e) {
-        const float d = value(r[i], e) - at, p = __builtin_amdgcn_exp2f(d * c);
+        const float y = (x[i][e] - ref) * c, p = __builtin_amdgcn_exp2f(y);
         s.z += p;
-        s.t = fmaf(p, fmaxf(d, -3e38f), s.t);  // (p is 0 where d is -infinity)
+        s.t = fmaf(p, fmaxf(y, -3e38f), s.t);  // (p is 0 where y is -infinity)
       }
     if (first) {
-      const float d = x_extra - at, p = __builtin_amdgcn_exp2f(d * c);
+      const float y = (x_extra - ref) * c, p = __builtin_amdgcn_exp2f(y);
       s.z += p;
-      s.t = fmaf(p, fmaxf(d, -3e38f), s.t);
+      s.t = fmaf(p, fmaxf(y, -3e38f), s.t);
     }
   };
 
@@ -333,9 +348,18 @@ DEV void logprob_part(const LogprobParams& P) {
   }
   if (tid < k) top[tid] = 0;
   __syncthreads();
-  s = Sums{sums[lane % W][0], sums[lane % W][1], sums[lane % W][2]};
+  {
+    float m = sums[0][0];
 #pragma unroll
-  for (int m = 1; m < W; m *= 2) s = join(s, Sums{shfl_xor(s.m, m), shfl_xor(s.z, m), shfl_xor(s.t, m)}, c);
+    for (int i = 1; i < W; ++i) m = fmaxf(m, sums[i][0]);
+    s = Sums{m, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const Sums o = refer(Sums{sums[i][0], sums[i][1], sums[i][2]}, m, c);
+      s.z += o.z;
+      s.t += o.t;
+    }
+  }
   if (k > 0) {
     int at = 0, total = 0;
 #pragma unroll
@@ -346,7 +370,7 @@ DEV void logprob_part(const LogprobParams& P) {
     __syncthreads();
   }
   if (P.n_parts == 1) {
-    write_row<DT>(P, row, s, top);
+    write_row<DT>(P, row, s, top, x0);
     return;
   }
   const int64_t pr = (int64_t)row * P.n_parts + part;
@@ -363,17 +387,22 @@ DEV void logprob_join(const LogprobParams& P) {
   __shared__ int count;
   const int tid = (int)threadIdx.x, lane = lane_id(), row = (int)blockIdx.x, k = P.n_top, n = P.n_parts * k;
   const float c = P.scale * kLog2e;
-  // every wave joins the sums by itself, one part a lane
+  // every wave joins the sums by itself, one part a lane; what the row needs of memory is
+  // asked for at once
   static_assert(kMaxLogitParts <= WAVE, "a part a lane");
+  constexpr int NT = kMaxLogitParts * kMaxTop / (WAVE * kLogitWaves);  // words of a thread
   const bool in_part = lane < P.n_parts;
   const float4 ps = reinterpret_cast<const float4*>(P.part_sums)[(int64_t)row * P.n_parts + (in_part ? lane : 0)];
   const uint64_t* in = P.part_top + (int64_t)row * n;
-  uint64_t least = 1;  // 0: no word
+  uint64_t least = 1, word[NT] = {};  // 0: no word
   if (k > 0) {
-    if (in_part) least = max(least, in[lane * k + k - 1]);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) word[i] = in[min(tid + i * WAVE * kLogitWaves, n - 1)];
+    least = max(least, in[(in_part ? lane : 0) * k + k - 1]);
     if (tid == 0) count = 0;
     if (tid < k) top[tid] = 0;
   }
+  const float x0 = tid < P.n_tokens ? token_logit<DT>(P, row, tid) : -kInf;
   const Sums s = wave_join(in_part ? Sums{ps.x, ps.y, ps.z} : Sums{-kInf, 0.0f, 0.0f}, c);
   if (k > 0) {
 #pragma unroll
@@ -382,20 +411,30 @@ DEV void logprob_join(const LogprobParams& P) {
       least = max(least, o);
     }
     __syncthreads();
-    for (int i = tid; i < n; i += (int)blockDim.x) {
-      const uint64_t x = in[i];
-      if (x >= least) words[atomicAdd(&count, 1)] = x;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const bool keep = tid + i * WAVE * kLogitWaves < n && word[i] >= least;
+      const uint64_t mask = __builtin_amdgcn_ballot_w64(keep);
+      if (mask == 0) continue;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&count, __builtin_popcountll(mask));
+      at = __builtin_amdgcn_readfirstlane(at);
+      if (keep) words[at + __builtin_popcountll(mask & ((1ull << lane) - 1))] = word[i];
     }
     __syncthreads();
     rank_words(words, count, k, top);
     __syncthreads();
   }
-  write_row<DT>(P, row, s, top);
+  write_row<DT>(P, row, s, top, x0);
 }
 
 }  // namespace
 
+#define VK_FOUR_WAVES __attribute__((amdgpu_waves_per_eu(4)))
 #define VK_LOGITS(DT)                                                                                                             \
-  extern "C" __global__ void __launch_bounds__(WAVE* kLogitWaves) vk_logprob_part_q##DT(const LogprobParams P) { logprob_part<DT>(P); } \
+  extern "C" __global__ void __launch_bounds__(WAVE* kLogitWaves) VK_FOUR_WAVES vk_logprob_part_q##DT(const LogprobParams P) {       \
+    logprob_part<DT, kLogitWaves>(P);                                                                                               \
+  }                                                                                                                                 \
+  extern "C" __global__ void __launch_bounds__(1024) vk_logprob_row_q##DT(const LogprobParams P) { logprob_part<DT, 16>(P); }        \
   extern "C" __global__ void __launch_bounds__(WAVE* kLogitWaves) vk_logprob_join_q##DT(const LogprobParams P) { logprob_join<DT>(P); }
 VK_LOGITS(0) VK_LOGITS(1)
