@@ -278,6 +278,7 @@ struct SelectParams {
   int32_t n_chunks;         // vk_page_scores: workgroups that share a (sequence, KV head)'s pages
 };
 constexpr int kSelWaves = 8;      // waves of a workgroup of the selection
+constexpr int kSelMaxWaves = 16;  // and of one that selects among keys in memory
 constexpr int kSelPages = 8192;   // pages whose scores vk_page_select holds in LDS
 struct SparseParams {
   const uint8_t* kc;

@@ -84,10 +84,11 @@ int plan_sparse(const vk_ctx* ctx, const vk_pool* pool, const vk_sparse_args* a,
   pl->units = (uint64_t)a->n_seqs * d.n_kv_heads;
   pl->max_pages = (int)(((int64_t)a->max_context_len + d.block_size - 1) / d.block_size);
   const int64_t units = std::max<int64_t>(1, (int64_t)pl->units);
-  // selection: one workgroup per (sequence, KV head), or several and a second launch
+  // selection: one workgroup per (sequence, KV head), or several and a second launch, which
+  // takes longer than 2048 pages of a CU do
   pl->n_chunks = 0;
   pl->select_bytes = 0;
-  if (pl->max_pages > kSelPages) {
+  if (pl->max_pages > kSelPages || (pl->max_pages > 2048 && 8 * units <= ctx->n_cu)) {
     constexpr int kChunk = 64 * kSelWaves;
     pl->n_chunks = (int)std::max<int64_t>(1, std::min<int64_t>((2 * ctx->n_cu + units - 1) / units, (pl->max_pages + kChunk - 1) / kChunk));
     pl->select_bytes = align_up(pl->units * pl->max_pages * sizeof(uint32_t), 256);
@@ -107,7 +108,7 @@ int plan_sparse(const vk_ctx* ctx, const vk_pool* pool, const vk_sparse_args* a,
     pl->ml_bytes = align_up(rows * 2 * sizeof(float), 256);
   }
   const uint64_t rows = ((uint64_t)a->n_seqs * a->n_heads + 3) / 4;
-  if (std::max({pl->units * std::max(1, pl->n_chunks) * 64 * kSelWaves, pl->units * pl->n_splits * 64 * pl->waves, rows * 256}) > kMaxThreads)
+  if (std::max({pl->units * std::max(2, pl->n_chunks) * 64 * kSelWaves, pl->units * pl->n_splits * 64 * pl->waves, rows * 256}) > kMaxThreads)
     return fail(VK_ERR_UNSUPPORTED, "grid too large");
   return VK_OK;
 }
@@ -138,12 +139,16 @@ int run_select(vk_ctx* ctx, vk_key_index* index, const vk_sparse_args* a, const 
   p.n_last = a->n_last;
   p.io_hd = pool->geom.io_hd;
   p.n_chunks = pl.n_chunks;
-  const dim3 threads(64 * kSelWaves), units((unsigned)pl.units);
-  if (!pl.n_chunks) return launch(ctx, select_name("vk_page_select", pool, pl.group, a->q_dtype).c_str(), units, threads, p, stream);
+  const dim3 threads(64 * kSelWaves), wide(64 * kSelMaxWaves), units((unsigned)pl.units);
+  if (!pl.n_chunks) {
+    // by rows where the workgroups are fewer than the CUs (velokv_sparse.hip, PageTurn)
+    const char* stage = pl.units < (uint64_t)ctx->n_cu ? "vk_page_select_rows" : "vk_page_select";
+    return launch(ctx, select_name(stage, pool, pl.group, a->q_dtype).c_str(), units, threads, p, stream);
+  }
   if (int rc = launch(ctx, select_name("vk_page_scores", pool, pl.group, a->q_dtype).c_str(),
                       dim3((unsigned)(pl.units * pl.n_chunks)), threads, p, stream))
     return rc;
-  return launch(ctx, "vk_page_topk", units, threads, p, stream);
+  return launch(ctx, "vk_page_topk", units, wide, p, stream);
 }
 
 int run_attend(vk_ctx* ctx, vk_pool* pool, const vk_sparse_args* a, const SparsePlan& pl, uint8_t* ws, void* stream) {
@@ -212,7 +217,7 @@ std::vector<std::string> velokv::sparse_kernel_names() {
     for (int kv = 0; kv < 4; ++kv) names.push_back("vk_index_update_kv" + std::to_string(kv) + w);
     for (int group : {16, 32})
       for (int qt : {VK_DT_F32, VK_DT_F16}) {
-        for (const char* stage : {"vk_page_select", "vk_page_scores"}) names.push_back(stage + std::string(w) + rows_tag(group, qt));
+        for (const char* stage : {"vk_page_select", "vk_page_select_rows", "vk_page_scores"}) names.push_back(stage + std::string(w) + rows_tag(group, qt));
         for (int kv = 0; kv < 4; ++kv) names.push_back("vk_sparse_kv" + std::to_string(kv) + w + rows_tag(group, qt));
       }
   }

@@ -284,7 +284,7 @@ DEV void index_read(const IndexReadParams& P) {
 // fit LDS one workgroup computes them and selects (vk_page_select); longer contexts,
 // and long ones of few sequences, are scored by several workgroups that leave the
 // keys in memory (vk_page_scores) for a second launch (vk_page_topk).
-constexpr int kSelThreads = 64 * kSelWaves;
+// W: waves of the workgroup.
 
 // What a workgroup of the selection knows of its (sequence, KV head).
 struct SelUnit {
@@ -336,43 +336,80 @@ DEV void load_query_codes(const SelectParams& P, const SelUnit& u, int8_t (*qc)[
 }
 
 // A wave's turn of 64 scored pages: their ids, codes and scales. keys[i] is page u.lo + i.
-template <int T>
+// Codes are loaded in the operands' order, or BY_ROW, a row by adjacent lanes (LPR each),
+// and change lanes in LDS. A CU takes 36 GB/s in the operands' order, where adjacent lanes
+// read 16 rows, and 95 by rows, so few (sequence, KV head)s load by rows (one sequence of
+// 375 pages x 8 heads: 7.5 us against 8.5, 8 of 512: 8.9 against 10.2); all CUs together
+// reach HBM's rate either way, and the operands' order takes fewer registers and no LDS
+// (64 sequences of 512 pages: 18.4 us against 19.6, 32 of 2048: 36.7 against 40).
+template <int T, bool BY_ROW>
 struct PageTurn {
-  static constexpr int KJ = 2 * T / 64;  // products of 64 dims
-  int raw;          // the lane's page id
-  i32x4 kb[4][KJ];  // codes of page 16 v + n, as operands
+  static constexpr int KJ = 2 * T / 64;                                         // products of 64 dims
+  static constexpr int LPR = 2 * T / 16, RPL = WAVE / LPR, NL = WAVE / RPL;  // lanes a row, rows a load, loads
+  int raw;              // the lane's page id
+  u32x4 codes[NL];      // by rows: chunk lane % LPR of page i RPL + lane / LPR; else chunk 4 (i % KJ) + g of page 16 (i / KJ) + n
   float scale;
 };
-DEV int page_id(const SelectParams& P, const SelUnit& u, int p) { return u.bt[u.lo + min(p + lane_id(), u.n - 1)]; }
+// LDS of one wave: 16 rows of 2 T codes, a row's 16-byte chunks in an order of its own so
+// that reads of one chunk of all rows meet all banks.
 template <int T>
-DEV void load_turn(const SelectParams& P, const SelUnit& u, int raw, PageTurn<T>& t) {
-  const int lane = lane_id(), n = lane & 15, g = lane >> 4;
-  const int page = min(max(raw, 0), P.n_pool_pages - 1);
+struct RowTile {
+  u32x4 c[16][2 * T / 16];
+  DEV static int place(int row, int chunk) { return chunk ^ (row & (2 * T / 16 - 1)); }
+};
+DEV int page_id(const SelectParams& P, const SelUnit& u, int p) { return u.bt[u.lo + min(p + lane_id(), u.n - 1)]; }
+template <int T, bool BY_ROW>
+DEV void load_turn(const SelectParams& P, const SelUnit& u, int raw, PageTurn<T, BY_ROW>& t) {
+  using Turn = PageTurn<T, BY_ROW>;
+  const int lane = lane_id(), n = lane & 15, g = lane >> 4, page = min(max(raw, 0), P.n_pool_pages - 1);
   t.raw = raw;
+  if constexpr (BY_ROW) {
 #pragma unroll
-  for (int v = 0; v < 4; ++v) {
-    const int64_t at = (int64_t)__shfl(page, 16 * v + n, WAVE) * P.n_kv_heads + u.kvh;
-    const i32x4* c = reinterpret_cast<const i32x4*>(P.codes + at * 2 * T + 16 * g);
+    for (int i = 0; i < Turn::NL; ++i) {
+      const int64_t at = (int64_t)__shfl(page, i * Turn::RPL + lane / Turn::LPR, WAVE) * P.n_kv_heads + u.kvh;
+      t.codes[i] = *reinterpret_cast<const u32x4*>(P.codes + at * 2 * T + 16 * (lane % Turn::LPR));
+    }
+  } else {
 #pragma unroll
-    for (int j = 0; j < PageTurn<T>::KJ; ++j) t.kb[v][j] = c[4 * j];
+    for (int v = 0; v < 4; ++v) {
+      const int64_t at = (int64_t)__shfl(page, 16 * v + n, WAVE) * P.n_kv_heads + u.kvh;
+      const u32x4* c = reinterpret_cast<const u32x4*>(P.codes + at * 2 * T + 16 * g);
+#pragma unroll
+      for (int j = 0; j < Turn::KJ; ++j) t.codes[v * Turn::KJ + j] = c[4 * j];
+    }
   }
   t.scale = P.scales[(int64_t)page * P.n_kv_heads + u.kvh];
+}
+// Pages 16 v .. 16 v + 15 of a turn as operands: chunk 4 j + g of page n.
+template <int T, bool BY_ROW>
+DEV void turn_operands(const PageTurn<T, BY_ROW>& t, int v, RowTile<T>* tile, i32x4 (&kb)[2 * T / 64]) {
+  using Turn = PageTurn<T, BY_ROW>;
+  const int lane = lane_id(), n = lane & 15, g = lane >> 4, r = lane / Turn::LPR, c = lane % Turn::LPR;
+  if constexpr (BY_ROW) {
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < Turn::NL / 4; ++i) tile->c[i * Turn::RPL + r][RowTile<T>::place(i * Turn::RPL + r, c)] = t.codes[v * (Turn::NL / 4) + i];
+    __builtin_amdgcn_wave_barrier();
+  }
+#pragma unroll
+  for (int j = 0; j < Turn::KJ; ++j) kb[j] = bitcast<i32x4>(BY_ROW ? tile->c[n][RowTile<T>::place(n, 4 * j + g)] : t.codes[v * Turn::KJ + j]);
 }
 
 // Keys of scored pages first, first + step, ..: 64 a turn, as four products of 16 pages
 // (the pages are the columns, the heads the rows). The first turn's loads are issued
 // before the queries' codes are made. Returns the lane's least and largest key.
-template <int QT, int T, int RT>
-DEV uint2 score_pages(const SelectParams& P, const SelUnit& u, int8_t (*qc)[2 * T], float* qs, int first, int step, uint32_t* keys) {
-  constexpr int KJ = PageTurn<T>::KJ;
+template <int QT, int T, int RT, bool BY_ROW>
+DEV uint2 score_pages(const SelectParams& P, const SelUnit& u, int8_t (*qc)[2 * T], float* qs, RowTile<T>* tile, int first,
+                      int step, uint32_t* keys) {
+  constexpr int KJ = 2 * T / 64;  // products of 64 dims
   const int lane = lane_id(), n = lane & 15, g = lane >> 4;
   uint2 span = make_uint2(0xFFFFFFFFu, 0u);
-  PageTurn<T> t;
+  PageTurn<T, BY_ROW> t;
   int next = 0;
   if (first < u.n) {
     const int raw = page_id(P, u, first);
     next = page_id(P, u, first + step);
-    load_turn<T>(P, u, raw, t);
+    load_turn<T, BY_ROW>(P, u, raw, t);
   }
   load_query_codes<QT, T, RT>(P, u, qc, qs);
   if (first >= u.n) return span;
@@ -392,12 +429,14 @@ DEV uint2 score_pages(const SelectParams& P, const SelUnit& u, int8_t (*qc)[2 * 
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const float sc = __shfl(t.scale, 16 * v + n, WAVE);
+      i32x4 kb[KJ];
+      turn_operands<T, BY_ROW>(t, v, tile, kb);
       best[v] = -kInf;  // a score that is not a number counts as this
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         i32x4 dot = {0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < KJ; ++j) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[rt][j], t.kb[v][j], dot, 0, 0, 0);
+        for (int j = 0; j < KJ; ++j) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[rt][j], kb[j], dot, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) best[v] = fmaxf(best[v], ((float)dot[i] * sc) * qsc[rt][i]);
       }
@@ -406,7 +445,7 @@ DEV uint2 score_pages(const SelectParams& P, const SelUnit& u, int8_t (*qc)[2 * 
     if (p0 + step < u.n) {
       const int raw = next;
       next = page_id(P, u, p0 + 2 * step);
-      load_turn<T>(P, u, raw, t);
+      load_turn<T, BY_ROW>(P, u, raw, t);
     }
     // the maximum over the row groups, which leaves lane l page p0 + l's
     swap_lanes<32>(best[0], best[2]);
@@ -449,19 +488,19 @@ DEV int wave_prefix_sum(int x) {
 // round's range. A bin of at most 64 keys is ranked by one wave.
 struct SelScratch {
   int hist[256];
-  int turn[kSelWaves][2];
+  int turn[kSelMaxWaves][2];
   uint32_t least, most, bin_keys[64];
   int n_bin, found[3];
 };
 DEV void select_begin(SelScratch& x) {  // before a barrier
   if (threadIdx.x == 0) { x.least = 0xFFFFFFFFu; x.most = 0; }
 }
-template <typename Keys>
+template <int W, typename Keys>
 DEV void select_top(const SelectParams& P, const SelUnit& u, const Keys keys, uint2 span, int32_t* pages, SelScratch& x) {
   const int tid = (int)threadIdx.x, lane = lane_id(), w = tid / WAVE;
   const int want_all = P.n_list - P.n_first - P.n_last;
-  for (int i = tid; i < P.n_first; i += kSelThreads) pages[i] = i;
-  for (int i = tid; i < P.n_last; i += kSelThreads) pages[P.n_list - P.n_last + i] = u.np - P.n_last + i;
+  for (int i = tid; i < P.n_first; i += W * WAVE) pages[i] = i;
+  for (int i = tid; i < P.n_last; i += W * WAVE) pages[P.n_list - P.n_last + i] = u.np - P.n_last + i;
   if (want_all == 0) return;
   const uint32_t least = ~wave_max_u(~span.x), most = wave_max_u(span.y);
   if (lane == 0) { atomicMin(&x.least, least); atomicMax(&x.most, most); }
@@ -475,7 +514,7 @@ DEV void select_top(const SelectParams& P, const SelUnit& u, const Keys keys, ui
     if (tid < 256) x.hist[tid] = 0;
     if (tid == 0) x.n_bin = 0;
     __syncthreads();
-    for (int i = tid; i < u.n; i += kSelThreads) {
+    for (int i = tid; i < u.n; i += W * WAVE) {
       const uint32_t k = keys[i] - base;
       if (bits == 32 || k >> bits == 0) atomicAdd(&x.hist[k >> shift], 1);
     }
@@ -509,7 +548,7 @@ DEV void select_top(const SelectParams& P, const SelUnit& u, const Keys keys, ui
     if (bits == 0) break;  // the bin is one key
     if (m > WAVE) { __syncthreads(); continue; }
     // the m keys of the bin: the want-th largest
-    for (int i = tid; i < u.n; i += kSelThreads) {
+    for (int i = tid; i < u.n; i += W * WAVE) {
       const uint32_t k = keys[i];
       if ((k - base) >> bits == 0) x.bin_keys[atomicAdd(&x.n_bin, 1)] = k;
     }
@@ -530,7 +569,7 @@ DEV void select_top(const SelectParams& P, const SelUnit& u, const Keys keys, ui
   __syncthreads();
   // a wave's share of the pages is one run of them, so that its place in the list follows
   // from how many the waves before it list
-  const int per = (u.n + kSelThreads - 1) / kSelThreads * WAVE;
+  const int per = (u.n + W * WAVE - 1) / (W * WAVE) * WAVE;
   const int i0 = w * per, i1 = min(u.n, i0 + per);
   int above = 0, equal = 0;
   for (int i = i0 + lane; i - lane < i1; i += WAVE) {
@@ -555,28 +594,35 @@ DEV void select_top(const SelectParams& P, const SelUnit& u, const Keys keys, ui
 }
 
 // A context of no more pages than the list has places: all of them.
+template <int W>
 DEV void list_all(const SelectParams& P, const SelUnit& u, int32_t* pages) {
-  for (int i = (int)threadIdx.x; i < P.n_list; i += kSelThreads) pages[i] = i < u.np ? i : -1;
+  for (int i = (int)threadIdx.x; i < P.n_list; i += W * WAVE) pages[i] = i < u.np ? i : -1;
 }
 
 // The wave's first page of a workgroup's chunk.
+constexpr int kSelThreads = kSelWaves * WAVE;
 DEV int first_page(int chunk) { return chunk * kSelThreads + __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE) * WAVE; }
 
-template <int QT, int T, int RT>
+template <int QT, int T, int RT, bool BY_ROW>
 DEV void page_select(const SelectParams& P) {
   __shared__ __align__(16) int8_t qc[16 * RT][2 * T];
   __shared__ float qs[16 * RT];
+  __shared__ RowTile<T> tiles[BY_ROW ? kSelWaves : 1];
   __shared__ uint32_t keys[kSelPages];
   __shared__ SelScratch scratch;
-  const SelUnit u = sel_unit(P, (int)blockIdx.x);
-  int32_t* pages = P.pages + (int64_t)blockIdx.x * P.n_list;
+  // each XCD takes a run of the units, so that the heads of a sequence, whose rows lie side by
+  // side, are read through one cache (64 sequences of 512 pages: 18.4 -> 17.5 us)
+  const int units = P.n_seqs * P.n_kv_heads, run = units / 8, b = (int)blockIdx.x;
+  const int unit = b < 8 * run ? (b & 7) * run + (b >> 3) : b;
+  const SelUnit u = sel_unit(P, unit);
+  int32_t* pages = P.pages + (int64_t)unit * P.n_list;
   if (u.n == 0) {
-    list_all(P, u, pages);
+    list_all<kSelWaves>(P, u, pages);
     return;
   }
   select_begin(scratch);
-  const uint2 span = score_pages<QT, T, RT>(P, u, qc, qs, first_page(0), kSelThreads, keys);
-  select_top(P, u, keys, span, pages, scratch);
+  const uint2 span = score_pages<QT, T, RT, BY_ROW>(P, u, qc, qs, &tiles[BY_ROW ? threadIdx.x / WAVE : 0], first_page(0), kSelThreads, keys);
+  select_top<kSelWaves>(P, u, keys, span, pages, scratch);
 }
 
 template <int QT, int T, int RT>
@@ -586,25 +632,26 @@ DEV void page_scores(const SelectParams& P) {
   const int chunk = (int)(blockIdx.x % P.n_chunks), unit = (int)(blockIdx.x / P.n_chunks);
   const SelUnit u = sel_unit(P, unit);
   if (chunk * kSelThreads >= u.n) return;
-  score_pages<QT, T, RT>(P, u, qc, qs, first_page(chunk), P.n_chunks * kSelThreads, P.keys + (int64_t)unit * P.max_pages);
+  score_pages<QT, T, RT, false>(P, u, qc, qs, nullptr, first_page(chunk), P.n_chunks * kSelThreads, P.keys + (int64_t)unit * P.max_pages);
 }
+template <int W>
 DEV void page_topk(const SelectParams& P) {
   __shared__ SelScratch scratch;
   const SelUnit u = sel_unit(P, (int)blockIdx.x);
   int32_t* pages = P.pages + (int64_t)blockIdx.x * P.n_list;
   if (u.n == 0) {
-    list_all(P, u, pages);
+    list_all<W>(P, u, pages);
     return;
   }
   const uint32_t* keys = P.keys + (int64_t)blockIdx.x * P.max_pages;
   select_begin(scratch);
   uint2 span = make_uint2(0xFFFFFFFFu, 0u);
-  for (int i = (int)threadIdx.x; i < u.n; i += kSelThreads) {
+  for (int i = (int)threadIdx.x; i < u.n; i += W * WAVE) {
     const uint32_t k = keys[i];
     span = make_uint2(min(span.x, k), max(span.y, k));
   }
   __syncthreads();
-  select_top(P, u, keys, span, pages, scratch);
+  select_top<W>(P, u, keys, span, pages, scratch);
 }
 
 // =============================================================================
@@ -1011,12 +1058,15 @@ DEV void sparse_merge(const SparseParams& P) {
 VK_INDEX(0) VK_INDEX(1) VK_INDEX(2) VK_INDEX(3)
 VK_KERNEL(vk_index_read, 256, IndexReadParams, index_read(P))
 
-#define VK_SELECT(TAG, QT, T, RT)                                                             \
-  VK_KERNEL(vk_page_select##TAG, kSelThreads, SelectParams, (page_select<QT, T, RT>(P)))       \
+#define VK_SELECT(TAG, QT, T, RT)                                                                       \
+  VK_KERNEL(vk_page_select##TAG, kSelThreads, SelectParams, (page_select<QT, T, RT, false>(P)))          \
+  VK_KERNEL(vk_page_select_rows##TAG, kSelThreads, SelectParams, (page_select<QT, T, RT, true>(P)))      \
   VK_KERNEL(vk_page_scores##TAG, kSelThreads, SelectParams, (page_scores<QT, T, RT>(P)))
-VK_SELECT(_r1_q0, 0, 128, 1) VK_SELECT(_r2_q0, 0, 128, 2) VK_SELECT(_d64_r1_q0, 0, 64, 1) VK_SELECT(_d64_r2_q0, 0, 64, 2)
-VK_SELECT(_r1_q1, 1, 128, 1) VK_SELECT(_r2_q1, 1, 128, 2) VK_SELECT(_d64_r1_q1, 1, 64, 1) VK_SELECT(_d64_r2_q1, 1, 64, 2)
-VK_KERNEL(vk_page_topk, kSelThreads, SelectParams, page_topk(P))
+#define VK_SELECT_Q(QT)                                                   \
+  VK_SELECT(_r1_q##QT, QT, 128, 1) VK_SELECT(_r2_q##QT, QT, 128, 2)          \
+  VK_SELECT(_d64_r1_q##QT, QT, 64, 1) VK_SELECT(_d64_r2_q##QT, QT, 64, 2)
+VK_SELECT_Q(0) VK_SELECT_Q(1)
+VK_KERNEL(vk_page_topk, 64 * kSelMaxWaves, SelectParams, page_topk<kSelMaxWaves>(P))
 
 #define VK_SPARSE(KV, QT)                                                                                          \
   VK_KERNEL(vk_sparse_kv##KV##_r1_q##QT, 64 * kSparseMaxWaves, SparseParams, (sparse_attn<KV, QT, 128, 1>(P)))         \
