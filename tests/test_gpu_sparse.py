@@ -154,6 +154,7 @@ def test_index_of_special_keys(ctx, kv):
 
 def choose(c, q, lens, rows, n_list, n_first, n_last):
     """Lists [S][Hkv][n_list] from the pool's keys and q."""
+    known = {}  # a page's bounds, by what they depend on
     out = np.full((len(lens), c.hkv, n_list), -1, np.int32)
     g = q.shape[1] // c.hkv
     q_scale, q_inv = code_parts(q.astype(np.float32))
@@ -166,7 +167,10 @@ def choose(c, q, lens, rows, n_list, n_first, n_last):
         for h in range(c.hkv):
             score = np.zeros(pages, np.float32)
             for p in range(pages):
-                lo, hi, scale = bounds(c, rows[s], p, h, min(c.page, int(n) - p * c.page))
+                at = (rows[s], p, h, min(c.page, int(n) - p * c.page))
+                if at not in known:
+                    known[at] = bounds(c, *at)
+                lo, hi, scale = known[at]
                 x = code[s, h * g:(h + 1) * g]
                 dot = np.where(x < 0, x * lo.astype(np.int64), x * hi.astype(np.int64)).sum(-1)
                 score[p] = ((dot.astype(np.float32) * scale) * q_scale[s, h * g:(h + 1) * g]).max()
@@ -206,6 +210,30 @@ def test_select_pages(ctx, group, head_dim, page, kv, q_dtype):
         got = select(c, index, q, lens, rows, n_list, n_first, n_last)
         ref = choose(c, q, lens, rows, n_list, n_first, n_last)
         assert np.array_equal(got, ref), (n_list, n_first, n_last)
+
+
+@pytest.mark.parametrize("group,head_dim,page,kv", [(1, 128, 16, O.I8_BLK), (8, 64, 16, O.F16), (20, 96, 32, O.I8_REF), (24, 40, 16, O.F32)])
+def test_select_pages_of_many_rows(ctx, group, head_dim, page, kv):
+    """As many (row, KV head)s as CUs and more: the loads take another order. Queries of one table row at many
+    lengths among them (whole pages: the index's bounds hold)."""
+    c = Cache(ctx, kv, [70 * page, 9 * page + 1], head_dim=head_dim, page=page, seed=31)
+    index = velokv.KeyIndex(ctx, c.pool)
+    ctx.index_update(index, 0, **c.dev())
+    rows = [0] * 160 + [1] * 3
+    lens = [page * (1 + i % 70) for i in range(160)] + [int(c.lens[1])] * 3
+    q = queries(c, len(rows), 2 * group, np.float16)
+    for n_list in (7, 30):
+        assert np.array_equal(select(c, index, q, lens, rows, n_list), choose(c, q, lens, rows, n_list, 1, 1))
+
+
+def test_select_long_contexts_of_some(ctx):
+    """40 (row, KV head)s of up to 2500 pages: several turns of a wave, one launch."""
+    c = Cache(ctx, O.F16, [16 * 2500 - 5], n_kv_heads=2, head_dim=64, seed=32)
+    index = velokv.KeyIndex(ctx, c.pool)
+    ctx.index_update(index, 0, **c.dev())
+    lens = [16 * 2500 - 5] + [16 * (100 * i + 70) for i in range(1, 20)]
+    q = queries(c, 20, 4, np.float32)
+    assert np.array_equal(select(c, index, q, lens, [0] * 20, 100), choose(c, q, lens, [0] * 20, 100, 1, 1))
 
 
 def test_select_ties_and_special_scores(ctx):
@@ -303,6 +331,17 @@ def test_sparse_decode(ctx, kv, q_dtype, group, head_dim, page):
         assert np.all(got[[0, 6]] == 0)  # no context
     lists[:] = -1
     assert np.all(sparse(c, q, lists, lens, rows) == 0)
+
+
+@pytest.mark.parametrize("rows,group,head_dim", [(140, 4, 128), (270, 4, 128), (270, 3, 64)])
+@pytest.mark.parametrize("kv", KVS)
+def test_sparse_decode_many_rows(ctx, kv, rows, group, head_dim):
+    """More (row, KV head)s than CUs, and more than twice as many: a list is one workgroup's, of eight waves or four."""
+    c = Cache(ctx, kv, [16 * 20 + 3, 5], head_dim=head_dim, seed=33)
+    at, lens = [i % 2 for i in range(rows)], [int(c.lens[0]) - i if i % 2 == 0 else 5 for i in range(rows)]
+    q = queries(c, rows, 2 * group, np.float16)
+    lists = some_lists(c, lens, 15)
+    close(sparse(c, q, lists, lens, at), attend(c, q, lists, lens, at))
 
 
 @pytest.mark.parametrize("kv", KVS)

@@ -355,7 +355,7 @@ struct PageTurn {
 template <int T>
 struct RowTile {
   u32x4 c[16][2 * T / 16];
-  DEV static int place(int row, int chunk) { return chunk ^ (row & (2 * T / 16 - 1)); }
+  static __device__ __forceinline__ int place(int row, int chunk) { return chunk ^ (row & (2 * T / 16 - 1)); }
 };
 DEV int page_id(const SelectParams& P, const SelUnit& u, int p) { return u.bt[u.lo + min(p + lane_id(), u.n - 1)]; }
 template <int T, bool BY_ROW>

@@ -254,13 +254,13 @@ class Context:
                      first_tokens=None, max_tokens: int = 0, block_tables=None, bt_stride: int = 0, seq_rows=None,
                      stream=None):
         """vk_index_update: the bounds of the pages that hold positions first_tokens (None: 0) .. context_lens - 1."""
-        check(lib().vk_index_update(self.h, index.h, layer, _bptr(block_tables), bt_stride, _bptr(seq_rows),
-                                    _bptr(first_tokens), _bptr(context_lens), n_seqs, max_context_len, max_tokens,
+        check(lib().vk_index_update(self.h, index.h, layer, _addr(block_tables), bt_stride, _addr(seq_rows),
+                                    _addr(first_tokens), _addr(context_lens), n_seqs, max_context_len, max_tokens,
                                     _sptr(stream)))
 
     def index_read(self, index: "KeyIndex", layer: int, pages, n_pages: int, lower, upper, stream=None):
         """vk_index_read: lower and upper bounds of listed pages as fp32 [n_pages][n_kv_heads][head_dim]."""
-        check(lib().vk_index_read(self.h, index.h, layer, _bptr(pages), n_pages, _bptr(lower), _bptr(upper),
+        check(lib().vk_index_read(self.h, index.h, layer, _addr(pages), n_pages, _addr(lower), _addr(upper),
                                   _sptr(stream)))
 
     def select_pages(self, index: "KeyIndex", layer: int, q, q_dtype: int, pages, n_pages: int, context_lens,
@@ -269,18 +269,18 @@ class Context:
                      stream=None):
         """vk_select_pages: the n_pages best pages of each (sequence, KV head) by their bounds, ascending, into
         pages (int32 [n_seqs][n_kv_heads][n_pages], -1 after a list's end)."""
-        a = _capi.SparseArgs(layer, _bptr(q), q_dtype, None, _bptr(pages), n_pages, n_first, n_last,
-                             _bptr(block_tables), bt_stride, _bptr(seq_rows), _bptr(context_lens), n_seqs, n_heads,
-                             max_context_len, 0.0, _bptr(workspace), workspace_bytes)
+        a = _capi.SparseArgs(layer, _addr(q), q_dtype, None, _addr(pages), n_pages, n_first, n_last,
+                             _addr(block_tables), bt_stride, _addr(seq_rows), _addr(context_lens), n_seqs, n_heads,
+                             max_context_len, 0.0, _addr(workspace), workspace_bytes)
         check(lib().vk_select_pages(self.h, index.h, C.byref(a), _sptr(stream)))
 
     def sparse_decode(self, pool: "Pool", layer: int, q, q_dtype: int, out, pages, n_pages: int, context_lens,
                       n_seqs: int, n_heads: int, max_context_len: int, block_tables=None, bt_stride: int = 0,
                       seq_rows=None, scale: float = 0.0, workspace=None, workspace_bytes: int = 0, stream=None):
         """vk_sparse_decode: decode attention over the pages listed for each (sequence, KV head)."""
-        a = _capi.SparseArgs(layer, _bptr(q), q_dtype, _bptr(out), _bptr(pages), n_pages, 0, 0, _bptr(block_tables),
-                             bt_stride, _bptr(seq_rows), _bptr(context_lens), n_seqs, n_heads, max_context_len, scale,
-                             _bptr(workspace), workspace_bytes)
+        a = _capi.SparseArgs(layer, _addr(q), q_dtype, _addr(out), _addr(pages), n_pages, 0, 0, _addr(block_tables),
+                             bt_stride, _addr(seq_rows), _addr(context_lens), n_seqs, n_heads, max_context_len, scale,
+                             _addr(workspace), workspace_bytes)
         check(lib().vk_sparse_decode(self.h, pool.h, C.byref(a), _sptr(stream)))
 
     def select_decode(self, index: "KeyIndex", layer: int, q, q_dtype: int, out, pages, n_pages: int, context_lens,
@@ -288,9 +288,9 @@ class Context:
                       block_tables=None, bt_stride: int = 0, seq_rows=None, scale: float = 0.0, workspace=None,
                       workspace_bytes: int = 0, stream=None):
         """vk_select_decode: select_pages, then sparse_decode over its lists (which stay in pages)."""
-        a = _capi.SparseArgs(layer, _bptr(q), q_dtype, _bptr(out), _bptr(pages), n_pages, n_first, n_last,
-                             _bptr(block_tables), bt_stride, _bptr(seq_rows), _bptr(context_lens), n_seqs, n_heads,
-                             max_context_len, scale, _bptr(workspace), workspace_bytes)
+        a = _capi.SparseArgs(layer, _addr(q), q_dtype, _addr(out), _addr(pages), n_pages, n_first, n_last,
+                             _addr(block_tables), bt_stride, _addr(seq_rows), _addr(context_lens), n_seqs, n_heads,
+                             max_context_len, scale, _addr(workspace), workspace_bytes)
         check(lib().vk_select_decode(self.h, index.h, C.byref(a), _sptr(stream)))
 
     def sparse_workspace_bytes(self, pool: "Pool", n_seqs, n_heads, max_context_len, n_pages, bt_stride=0,
@@ -307,9 +307,9 @@ class Context:
                        row_stride: int = 0, scale: float = 0.0, workspace=None, workspace_bytes: int = 0, stream=None):
         """vk_token_logprobs: log probabilities of given tokens, entropy and the n_top most probable tokens of
         each row of logits."""
-        a = _capi.LogprobArgs(_bptr(logits), dtype, row_stride, n_rows, vocab, scale, _bptr(tokens), n_tokens,
-                              _bptr(token_logprobs), _bptr(entropy), _bptr(top_ids), _bptr(top_logprobs), n_top,
-                              _bptr(workspace), workspace_bytes)
+        a = _capi.LogprobArgs(_addr(logits), dtype, row_stride, n_rows, vocab, scale, _addr(tokens), n_tokens,
+                              _addr(token_logprobs), _addr(entropy), _addr(top_ids), _addr(top_logprobs), n_top,
+                              _addr(workspace), workspace_bytes)
         check(lib().vk_token_logprobs(self.h, C.byref(a), _sptr(stream)))
 
     def token_logprobs_workspace_bytes(self, n_rows: int, vocab: int, n_top: int = 0, dtype: int = DT_F16) -> int:
@@ -375,6 +375,11 @@ def _bptr(b):
     if isinstance(b, int):
         return C.c_void_p(b)
     return b
+
+
+def _addr(b):
+    """A buffer's address as ctypes takes it (None, an int or a c_void_p as they are)."""
+    return b.ptr if isinstance(b, DeviceBuffer) else b
 
 
 def _sptr(s):
