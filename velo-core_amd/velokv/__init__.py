@@ -5,8 +5,9 @@ paged_attention.rs:92-212, metal/runtime.rs:274-324): a HIP context, K/V pools
 in HBM with a slot block table, the block manager, and the three hot-path
 operations (append with INT8 quantization, paged decode attention, copy-on-write
 block copy) plus tree-verify attention, the accepted-path commit of a verified
-tree, and NIXL wire-record pack/unpack of KV pages. Every compute call goes to the gfx950
-code object through libvelokv.so.
+tree, NIXL wire-record pack/unpack of KV pages, sparse decode over pages chosen by a key
+index, and log probabilities of logits. Every compute call goes to the gfx950 code objects
+through libvelokv.so.
 """
 from ._capi import (  # noqa: F401
     DT_F16, DT_F32, DECODE_AUTO, DECODE_MFMA, DECODE_VALU, SCHED_AUTO, SCHED_SPLIT, SCHED_STREAM, SCHED_WORKGROUP, SCHED_PACKED, NOALLOC_SCRATCH_BYTES, KV_F16, KV_F32, KV_I8_BLK, KV_I8_REF, VkError,
