@@ -371,6 +371,17 @@ def test_sparse_decode_value_scales(ctx):
     close(sparse(c, q, lists, c.lens, [0]), attend(c, q, lists, c.lens, [0]))
 
 
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** -40])
+@pytest.mark.parametrize("kv", KVS)
+def test_sparse_decode_query_sizes(ctx, kv, size):
+    """fp32 queries past fp16's largest value and far below its least, one row's heads apart by 2^8."""
+    c = Cache(ctx, kv, [16 * 20 + 3], seed=35)
+    q = (queries(c, 1, 8, np.float32) * (size * 2.0 ** np.arange(0, -8, -1))[None, :, None]).astype(np.float32)
+    lists = some_lists(c, c.lens, 15)
+    scale = 1 / (size * math.sqrt(c.hd))
+    close(sparse(c, q, lists, c.lens, [0], scale=scale), attend(c, q, lists, c.lens, [0], scale))
+
+
 @pytest.mark.parametrize("kv", KVS)
 def test_what_lies_past_the_context(ctx, kv):
     """Infinite and NaN rows in the last page past the context do not reach the result."""

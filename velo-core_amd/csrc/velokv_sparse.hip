@@ -814,9 +814,10 @@ DEV void sparse_attn(const SparseParams& P) {
   // q^T: row n of each 16-row tile (rows past the group repeat its last one: their columns of
   // the results are not used), zeros past head_dim
   half8 qa[RT][F32 ? 1 : KC], qlo[RT][QSPLIT ? KC : 1];
-  float qf[RT][F32 ? T / 4 : 1];
+  float qf[RT][F32 ? T / 4 : 1], scale_log2[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
+    scale_log2[rt] = P.scale_log2;
     const int64_t off = (row0 + min(16 * rt + n, G - 1)) * P.io_hd;
     if constexpr (F32) {
 #pragma unroll
@@ -828,18 +829,32 @@ DEV void sparse_attn(const SparseParams& P) {
         for (int e = 0; e < 4; ++e) qf[rt][4 * j + e] = d < P.io_hd ? x[e] : 0.0f;
       }
     } else {
+      float x[KC][8], top = 0.0f;
 #pragma unroll
       for (int j = 0; j < KC; ++j) {
         const int d = sparse_qdim<KV, T>(j, g);
-        float x[8];
-        load_q<QT, 8>(P.q, off + min(d, P.io_hd - 8), x);
+        load_q<QT, 8>(P.q, off + min(d, P.io_hd - 8), x[j]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float v = d < P.io_hd ? x[i] : 0.0f;
+          x[j][i] = d < P.io_hd ? x[j][i] : 0.0f;
+          if constexpr (QSPLIT) top = fmaxf(top, fabsf(x[j][i]));
+        }
+      }
+      int up = 0;  // an fp32 row is taken times 2^up, which brings its largest to [2^13, 2^14): fp16 ends at 2^16
+      if constexpr (QSPLIT) {
+        top = fmaxf(top, shfl_xor(top, 16));
+        top = fmaxf(top, shfl_xor(top, 32));
+        up = top > 0.0f && top < kInf ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+        scale_log2[rt] = __builtin_amdgcn_ldexpf(P.scale_log2, -up);
+      }
+#pragma unroll
+      for (int j = 0; j < KC; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float v = QSPLIT ? __builtin_amdgcn_ldexpf(x[j][i], up) : x[j][i];
           qa[rt][j][i] = (_Float16)v;
           if constexpr (QSPLIT) qlo[rt][j][i] = (_Float16)(v - (float)qa[rt][j][i]);
         }
-      }
     }
   }
 
@@ -899,9 +914,9 @@ DEV void sparse_attn(const SparseParams& P) {
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float v = sc[i] * P.scale_log2, up = 0.0f;
-          if constexpr (BLK) { v = sc[i] * st[u].ks[0] * P.scale_log2; up = __builtin_amdgcn_logf(fmaxf(st[u].vs[0], kMinScale)); }
-          if constexpr (REF) { v = sc[i] * st[u].ks[i] * P.scale_log2; up = __builtin_amdgcn_logf(fmaxf(st[u].vs[i], kMinScale)); }
+          float v = sc[i] * scale_log2[rt], up = 0.0f;
+          if constexpr (BLK) { v = sc[i] * st[u].ks[0] * scale_log2[rt]; up = __builtin_amdgcn_logf(fmaxf(st[u].vs[0], kMinScale)); }
+          if constexpr (REF) { v = sc[i] * st[u].ks[i] * scale_log2[rt]; up = __builtin_amdgcn_logf(fmaxf(st[u].vs[i], kMinScale)); }
           x[u][i] = 4 * g + i < st[u].n_tok ? v : -kInf;
           top = fmaxf(top, x[u][i] + up);
         }
