@@ -85,6 +85,17 @@ DEV float sum_same_quadpos(float x) {
 DEV float readlane_f(float x, int l) { return bitcast<float>(__builtin_amdgcn_readlane(bitcast<int>(x), l)); }
 DEV int readlane_i(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
 
+template <int CTRL>
+DEV uint32_t dpp_u(uint32_t x, uint32_t old) { return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)x, CTRL, 0xF, 0xF, false); }
+DEV uint32_t wave_max_u(uint32_t x) {
+  x = max(x, dpp_u<DPP_QUAD_XOR1>(x, x));
+  x = max(x, dpp_u<DPP_QUAD_XOR2>(x, x));
+  x = max(x, dpp_u<DPP_ROW_HALF_MIRROR>(x, x));
+  x = max(x, dpp_u<DPP_ROW_MIRROR>(x, x));
+  return max(max((uint32_t)readlane_i((int)x, 0), (uint32_t)readlane_i((int)x, 16)),
+             max((uint32_t)readlane_i((int)x, 32), (uint32_t)readlane_i((int)x, 48)));
+}
+
 // A float as an unsigned key of the same order (-0 as 0; not for NaN), and back.
 DEV uint32_t order_key(float x) {
   const uint32_t u = bitcast<uint32_t>(x + 0.0f);

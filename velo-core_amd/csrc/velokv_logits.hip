@@ -120,14 +120,19 @@ DEV void write_row(const LogprobParams& P, int row, const Sums& s, const uint64_
   }
 }
 
-// Sorts words into top[0 .. k), largest first: each word's place is the number of larger ones.
+// Sorts words into top[0 .. k), largest first: each word's place is the number of larger
+// ones. Eight lanes a word, which divide the others.
 DEV void rank_words(const uint64_t* words, int n, int k, uint64_t* top) {
-  for (int i = (int)threadIdx.x; i < n; i += (int)blockDim.x) {
+  const int sub = (int)threadIdx.x & 7;
+  for (int i = (int)threadIdx.x >> 3; i < n; i += (int)blockDim.x >> 3) {
     const uint64_t x = words[i];
     int place = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) place += words[j] > x;
-    if (place < k) top[place] = x;
+#pragma unroll 2
+    for (int j = sub; j < n; j += 8) place += words[j] > x;
+    place += (int)dpp_u<DPP_QUAD_XOR1>((uint32_t)place, 0);
+    place += (int)dpp_u<DPP_QUAD_XOR2>((uint32_t)place, 0);
+    place += (int)dpp_u<DPP_ROW_HALF_MIRROR>((uint32_t)place, 0);
+    if (sub == 0 && place < k) top[place] = x;
   }
 }
 
@@ -142,7 +147,8 @@ DEV void logprob_part(const LogprobParams& P) {
   __shared__ uint64_t lists[W][kList];
   __shared__ uint64_t words[W * kMaxTop];
   __shared__ uint64_t top[kMaxTop];
-  __shared__ float sums[W][3], group_max[32];
+  __shared__ float sums[W][3];
+  __shared__ __align__(16) float group_max[32];
   __shared__ int counts[W];
   const int tid = (int)threadIdx.x, lane = lane_id(), w = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int row = (int)(blockIdx.x / P.n_parts), part = (int)(blockIdx.x % P.n_parts);
@@ -233,9 +239,13 @@ DEV void logprob_part(const LogprobParams& P) {
         __syncthreads();
         const float mine = group_max[lane & 31];
         if (k > 1) {  // the largest that k of them reach
-          int reach = 0;
+          int reach = 0;  // lanes 32 apart hold the same group and count half of them each
 #pragma unroll
-          for (int j = 0; j < 32; ++j) reach += readlane_f(mine, j) >= mine;
+          for (int j = 0; j < 4; ++j) {
+            const float4 o = reinterpret_cast<const float4*>(group_max)[4 * (lane >> 5) + j];
+            reach += (o.x >= mine) + (o.y >= mine) + (o.z >= mine) + (o.w >= mine);
+          }
+          reach += __float_as_int(xor32(__int_as_float(reach)));
           thr_x = wave_max(reach >= k ? mine : -kInf);
         } else {
           thr_x = wave_max(mine);
@@ -378,8 +388,7 @@ DEV void logprob_part(const LogprobParams& P) {
   if (tid < k) P.part_top[pr * k + tid] = top[tid];
 }
 
-// The parts of a row. A word can be among the k largest only if it reaches the largest
-// of the parts' k-th words.
+// The parts of a row.
 template <int DT>
 DEV void logprob_join(const LogprobParams& P) {
   __shared__ uint64_t words[kMaxLogitParts * kMaxTop];
@@ -394,22 +403,26 @@ DEV void logprob_join(const LogprobParams& P) {
   const bool in_part = lane < P.n_parts;
   const float4 ps = reinterpret_cast<const float4*>(P.part_sums)[(int64_t)row * P.n_parts + (in_part ? lane : 0)];
   const uint64_t* in = P.part_top + (int64_t)row * n;
-  uint64_t least = 1, word[NT] = {};  // 0: no word
+  // the need-th largest of the parts' at_least-th words is reached by need x at_least >= k
+  // words, of the parts' k each; some half more than k reach it
+  const int at_least = min(k, (5 * k + 4 * P.n_parts - 1) / (4 * P.n_parts)), need = (k + at_least - 1) / max(at_least, 1);
+  uint32_t nth = 0;
+  uint64_t word[NT] = {};  // 0: no word
   if (k > 0) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) word[i] = in[min(tid + i * WAVE * kLogitWaves, n - 1)];
-    least = max(least, in[(in_part ? lane : 0) * k + k - 1]);
+    nth = (uint32_t)(in[(in_part ? lane : 0) * k + at_least - 1] >> 32);
     if (tid == 0) count = 0;
     if (tid < k) top[tid] = 0;
   }
   const float x0 = tid < P.n_tokens ? token_logit<DT>(P, row, tid) : -kInf;
   const Sums s = wave_join(in_part ? Sums{ps.x, ps.y, ps.z} : Sums{-kInf, 0.0f, 0.0f}, c);
   if (k > 0) {
+    int reach = 0;
+    for (int j = 0; j < P.n_parts; j += 8)
 #pragma unroll
-    for (int m = 1; m < WAVE; m *= 2) {
-      const uint64_t o = (uint64_t)(uint32_t)__shfl_xor((int)(least >> 32), m, WAVE) << 32 | (uint32_t)__shfl_xor((int)least, m, WAVE);
-      least = max(least, o);
-    }
+      for (int e = 0; e < 8; ++e) reach += j + e < P.n_parts && (uint32_t)readlane_i((int)nth, j + e) >= nth;
+    const uint64_t least = max(1ull, (uint64_t)wave_max_u(in_part && reach >= need ? nth : 0u) << 32);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NT; ++i) {

@@ -49,9 +49,6 @@ DEV void swap_lanes(float& x, float& y) {
   x = bitcast<float>(a);
   y = bitcast<float>(b);
 }
-template <int CTRL>
-DEV uint32_t dpp_u(uint32_t x, uint32_t old) { return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)x, CTRL, 0xF, 0xF, false); }
-
 // Bounds of dims as signed integers, one (fp32) or two (PK: 16 bits each) a word.
 // Integers take one instruction a comparison; a float minimum of a value from another
 // lane takes two.
@@ -463,14 +460,6 @@ DEV uint2 score_pages(const SelectParams& P, const SelUnit& u, int8_t (*qc)[2 * 
   return span;
 }
 
-DEV uint32_t wave_max_u(uint32_t x) {
-  x = max(x, dpp_u<DPP_QUAD_XOR1>(x, x));
-  x = max(x, dpp_u<DPP_QUAD_XOR2>(x, x));
-  x = max(x, dpp_u<DPP_ROW_HALF_MIRROR>(x, x));
-  x = max(x, dpp_u<DPP_ROW_MIRROR>(x, x));
-  return max(max((uint32_t)readlane_i((int)x, 0), (uint32_t)readlane_i((int)x, 16)),
-             max((uint32_t)readlane_i((int)x, 32), (uint32_t)readlane_i((int)x, 48)));
-}
 // Sum over lanes 0 .. l.
 DEV int wave_prefix_sum(int x) {
   x += (int)dpp_u<0x111>((uint32_t)x, 0);  // row_shr 1, 2, 4, 8
