@@ -574,7 +574,8 @@ int vk_select_pages(vk_ctx* ctx, vk_key_index* index, const vk_sparse_args* a, v
  * past the context name nothing; a page listed twice counts twice; rows with no
  * token are 0. a->n_first and a->n_last are checked, not used. Results are those of
  * fp32 arithmetic over the stored values to about 2^-20 of the largest, whatever the
- * types. */
+ * types. With a query or a listed key that is not finite the row is unspecified (in
+ * bounds, no other row is affected); so is the dim of a listed value that is not. */
 int vk_sparse_decode(vk_ctx* ctx, vk_pool* pool, const vk_sparse_args* a, void* stream);
 
 /* vk_select_pages, then vk_sparse_decode over its lists, on one stream. */

@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 
 import velokv
+from test_gpu_sparse import Graph
 from velokv import synth
 
 pytestmark = pytest.mark.gpu
@@ -138,6 +139,50 @@ def test_many_tokens_and_no_entropy(ctx):
     x, _ = some(2, 9000, np.float16, seed=9)
     tokens = synth.rng(2).integers(0, 9000, (2, 700)).astype(np.int32)
     check(run(ctx, x, tokens, 2, entropy=False), x, tokens, 2)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("parts", [5, 9, 32])
+def test_alternatives_of_uneven_parts(ctx, dtype, parts):
+    """Rows of several parts whose largest values lie in one part, in the last few values, in order, or are equal."""
+    vocab, r = 8192 * parts - 8190, synth.rng(parts)  # the last part: two values
+    x = r.standard_normal((8, vocab)).astype(dtype)
+    x[0, 8192:16384] += dtype(8)
+    x[1, -3:] = 20
+    x[2] = np.sort(x[2])
+    x[3] = np.sort(x[3])[::-1]
+    x[4] = 1
+    x[5] = r.integers(0, 2, vocab)
+    x[6] = -np.inf
+    x[6, [5, 9000, vocab - 1]] = [1, 2, 3]
+    x[7] = r.integers(0, 40, vocab)
+    tokens = r.integers(0, vocab, (8, 1)).astype(np.int32)
+    for n_top in (1, 2, 7, 20, 31, 32):
+        check(run(ctx, x, tokens, n_top), x, tokens, n_top)
+
+
+def test_captured_calls_replay(ctx):
+    """A call in parts with a workspace of its own, replayed as the logits change, beside eager calls."""
+    rows, vocab, n_top = 3, 100000, 5
+    need = ctx.token_logprobs_workspace_bytes(rows, vocab, n_top)
+    x, tokens = some(rows, vocab, np.float16, seed=11)
+    dx, dt, ws, stream = ctx.upload(x), ctx.upload(tokens), ctx.alloc(need), velokv.Stream(ctx)
+    outs = dict(token_logprobs=ctx.alloc(tokens.size * 4), top_ids=ctx.alloc(rows * n_top * 4),
+                top_logprobs=ctx.alloc(rows * n_top * 4), entropy=ctx.alloc(rows * 4))
+    shapes = dict(token_logprobs=tokens.shape, top_ids=(rows, n_top), top_logprobs=(rows, n_top), entropy=(rows,))
+    ctx.sync()
+    with Graph(stream) as graph:
+        ctx.token_logprobs(dx, velokv.DT_F16, rows, vocab, tokens=dt, n_tokens=tokens.shape[1], n_top=n_top, workspace=ws,
+                           workspace_bytes=need, stream=stream, **outs)
+    for step in range(4):
+        x, tokens = some(rows, vocab, np.float16, seed=20 + step)
+        dx.upload(x)
+        dt.upload(tokens)
+        graph.replay()
+        check({k: o.download(shapes[k], np.int32 if k == "top_ids" else np.float32) for k, o in outs.items()}, x, tokens, n_top)
+        y, given = some(2, 50000, np.float32, seed=40 + step)
+        check(run(ctx, y, given, 3), y, given, 3)
+    graph.close()
 
 
 def test_workspace_and_streams(ctx):

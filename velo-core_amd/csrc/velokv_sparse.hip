@@ -33,6 +33,9 @@ DEV int to_code(float x, float inv) { return (int)fminf(fmaxf(rintf(x * inv), -1
 // fixed set of dims and the tokens' lanes are joined by lane exchanges at the end.
 // A page with a key that is not finite has the scale infinity (it is chosen before
 // any other).
+// Bound: the chain of table, keys and codes. The newest pages of 64 sequences x 8 heads
+// (fp16): 3.4 us; 4 int8 prompts of 1500-2500 tokens x 8 heads: 7.1 us for 9 MB. The
+// loads of a tile are all in flight at once.
 // =============================================================================
 // Exchanges x's lanes with bit M set and y's without: afterwards a lane without it
 // holds both halves of x, one with it both of y.
@@ -274,14 +277,18 @@ DEV void index_read(const IndexReadParams& P) {
 // 127 < 2^24: exact in fp32 too) and the score
 //     max over the group's heads of fp32(fp32(dot * page scale) * head scale)
 // has the same bits however it is computed. Scores are kept as ordered 32-bit keys
-// (larger key = chosen earlier); the pages that are always kept have the largest.
-// =============================================================================
+// (larger key = chosen earlier). The pages that are always kept are not scored.
 //
-// The pages that are always kept are not scored. Where a (sequence, KV head)'s scores
-// fit LDS one workgroup computes them and selects (vk_page_select); longer contexts,
-// and long ones of few sequences, are scored by several workgroups that leave the
-// keys in memory (vk_page_scores) for a second launch (vk_page_topk).
-// W: waves of the workgroup.
+// Where a (sequence, KV head)'s scores fit LDS one workgroup computes them and selects
+// (vk_page_select); longer contexts, and long ones of few sequences, are scored by
+// several workgroups that leave the keys in memory (vk_page_scores) for a second launch
+// (vk_page_topk).
+//
+// Bound: the rate at which rows of 2 T codes at unrelated addresses arrive. 64 sequences
+// of 512 pages x 8 heads (T = 128): 17.4 us, 69 MB at 4.0 TB/s, where a kernel of these
+// loads alone takes 12.5; 32 of 2048: 34.6 us, 136 MB, the loads alone 27. One sequence of
+// 375 pages: 7.4 us, of which an empty launch is 4.7.
+// =============================================================================
 
 // What a workgroup of the selection knows of its (sequence, KV head).
 struct SelUnit {
@@ -655,6 +662,10 @@ DEV void page_topk(const SelectParams& P) {
 // p enters it as two fp16 parts, p = hi + lo to 2^-22 relative (fp32 pools: fp32
 // throughout); the maximum is that of p times the value's scale, so that what is
 // rounded to fp16 lies in (0, 2^15].
+// Bound: HBM where the (sequence, KV head)s fill the CUs. 64 sequences of 64 listed
+// pages x 8 heads, fp16: 45.4 us, 270 MB at 6.0 TB/s; 32 of 128 pages, int8: 29 us, 4.6
+// TB/s with the launch and the chain of list, table and first tile. Few sequences: that
+// chain, then the merge (one sequence of 64 pages: 7.2 + 3.0 us).
 // =============================================================================
 constexpr float kShift = 11.0f;           // p is held times 2^11: fp16 subnormals begin 2^-36 below the largest
 constexpr float kRaise = 4.0f;            // the maximum is raised when a score passes it by 2^4
@@ -1012,7 +1023,7 @@ DEV void sparse_attn(const SparseParams& P) {
 }
 
 // Joins the parts of a row: one wave a row, T / 64 dims a lane; lane v holds part v's
-// maximum and sum, 64 parts a turn.
+// maximum and sum, 64 parts a turn. Bound: launch and one round of loads, 2.2-4 us.
 template <int T>
 DEV void sparse_merge(const SparseParams& P) {
   constexpr int EPL = T / WAVE, UN = 8;
