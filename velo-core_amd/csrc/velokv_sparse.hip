@@ -307,21 +307,31 @@ DEV SelUnit sel_unit(const SelectParams& P, int unit) {
   return u;
 }
 
-// Codes of the (sequence, KV head)'s queries in LDS, negative parts first; rows past
-// the group repeat its last one (their scores change no maximum). Ends with a barrier.
-template <int QT, int T, int RT>
-DEV void load_query_codes(const SelectParams& P, const SelUnit& u, int8_t (*qc)[2 * T], float* qs) {
+// Values of query row r of a (sequence, KV head): dims EPL l .. of lane l, rows past the
+// group as its last one.
+template <int QT, int T>
+DEV void load_query_row(const SelectParams& P, int unit, int r, float (&x)[T / WAVE]) {
+  constexpr int EPL = T / WAVE;
+  const int G = P.n_heads / P.n_kv_heads;
+  const int64_t row = ((int64_t)unit * G + min(r, G - 1)) * P.io_hd;
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) {
+    const int64_t at = row + min(lane_id() * EPL + e, P.io_hd - 1);
+    x[e] = QT == DT_F32 ? reinterpret_cast<const float*>(P.q)[at] : h2f(reinterpret_cast<const uint16_t*>(P.q)[at]);
+  }
+}
+// Codes of the (sequence, KV head)'s queries in LDS, negative parts first. x: row w of wave w,
+// which is loaded ahead of everything else. Ends with a barrier.
+template <int QT, int T>
+DEV void query_codes(const SelectParams& P, int unit, float (&x)[T / WAVE], int8_t (*qc)[2 * T], float* qs) {
   const int lane = lane_id(), w = (int)threadIdx.x / WAVE, G = P.n_heads / P.n_kv_heads;
   constexpr int EPL = T / WAVE;
-  for (int r = w; r < 16 * RT; r += kSelWaves) {
-    float x[EPL], bad = 0.0f, top = 0.0f;
-    const int64_t row = ((int64_t)u.s * P.n_heads + (int64_t)u.kvh * G + min(r, G - 1)) * P.io_hd;
+  for (int r = w; r < G; r += kSelWaves) {
+    if (r != w) load_query_row<QT, T>(P, unit, r, x);
+    float bad = 0.0f, top = 0.0f;
 #pragma unroll
     for (int e = 0; e < EPL; ++e) {
-      const int d = lane * EPL + e;
-      const int64_t at = row + min(d, P.io_hd - 1);
-      x[e] = QT == DT_F32 ? reinterpret_cast<const float*>(P.q)[at] : h2f(reinterpret_cast<const uint16_t*>(P.q)[at]);
-      x[e] = d < P.io_hd ? x[e] : 0.0f;
+      x[e] = lane * EPL + e < P.io_hd ? x[e] : 0.0f;
       top = fmaxf(top, fabsf(x[e]));
       bad = fmaf(x[e], 0.0f, bad);
     }
@@ -400,11 +410,12 @@ DEV void turn_operands(const PageTurn<T, BY_ROW>& t, int v, RowTile<T>* tile, i3
 }
 
 // Keys of scored pages first, first + step, ..: 64 a turn, as four products of 16 pages
-// (the pages are the columns, the heads the rows). The first turn's loads are issued
-// before the queries' codes are made. Returns the lane's least and largest key.
+// (the pages are the columns, the heads the rows; rows past the group repeat its last one,
+// whose scores change no maximum). The first turn's loads are issued before the queries'
+// codes are made. Returns the lane's least and largest key.
 template <int QT, int T, int RT, bool BY_ROW>
-DEV uint2 score_pages(const SelectParams& P, const SelUnit& u, int8_t (*qc)[2 * T], float* qs, RowTile<T>* tile, int first,
-                      int step, uint32_t* keys) {
+DEV uint2 score_pages(const SelectParams& P, const SelUnit& u, int unit, float (&x)[T / WAVE], int8_t (*qc)[2 * T], float* qs,
+                      RowTile<T>* tile, int first, int step, uint32_t* keys) {
   constexpr int KJ = 2 * T / 64;  // products of 64 dims
   const int lane = lane_id(), n = lane & 15, g = lane >> 4;
   uint2 span = make_uint2(0xFFFFFFFFu, 0u);
@@ -415,16 +426,17 @@ DEV uint2 score_pages(const SelectParams& P, const SelUnit& u, int8_t (*qc)[2 * 
     next = page_id(P, u, first + step);
     load_turn<T, BY_ROW>(P, u, raw, t);
   }
-  load_query_codes<QT, T, RT>(P, u, qc, qs);
+  query_codes<QT, T>(P, unit, x, qc, qs);
+  const int G = P.n_heads / P.n_kv_heads;
   if (first >= u.n) return span;
   i32x4 qa[RT][KJ];
   float qsc[RT][4];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
-    for (int j = 0; j < KJ; ++j) qa[rt][j] = *reinterpret_cast<const i32x4*>(&qc[16 * rt + n][64 * j + 16 * g]);
+    for (int j = 0; j < KJ; ++j) qa[rt][j] = *reinterpret_cast<const i32x4*>(&qc[min(16 * rt + n, G - 1)][64 * j + 16 * g]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) qsc[rt][i] = qs[16 * rt + 4 * g + i];
+    for (int i = 0; i < 4; ++i) qsc[rt][i] = qs[min(16 * rt + 4 * g + i, G - 1)];
   }
   bool out = false;
   for (int p0 = first; p0 < u.n; p0 += step) {
@@ -610,6 +622,8 @@ DEV void page_select(const SelectParams& P) {
   // side, are read through one cache (64 sequences of 512 pages: 18.4 -> 17.5 us)
   const int units = P.n_seqs * P.n_kv_heads, run = units / 8, b = (int)blockIdx.x;
   const int unit = b < 8 * run ? (b & 7) * run + (b >> 3) : b;
+  float x[T / WAVE];
+  load_query_row<QT, T>(P, unit, (int)threadIdx.x / WAVE, x);
   const SelUnit u = sel_unit(P, unit);
   int32_t* pages = P.pages + (int64_t)unit * P.n_list;
   if (u.n == 0) {
@@ -617,7 +631,7 @@ DEV void page_select(const SelectParams& P) {
     return;
   }
   select_begin(scratch);
-  const uint2 span = score_pages<QT, T, RT, BY_ROW>(P, u, qc, qs, &tiles[BY_ROW ? threadIdx.x / WAVE : 0], first_page(0), kSelThreads, keys);
+  const uint2 span = score_pages<QT, T, RT, BY_ROW>(P, u, unit, x, qc, qs, &tiles[BY_ROW ? threadIdx.x / WAVE : 0], first_page(0), kSelThreads, keys);
   select_top<kSelWaves>(P, u, keys, span, pages, scratch);
 }
 
@@ -626,9 +640,11 @@ DEV void page_scores(const SelectParams& P) {
   __shared__ __align__(16) int8_t qc[16 * RT][2 * T];
   __shared__ float qs[16 * RT];
   const int chunk = (int)(blockIdx.x % P.n_chunks), unit = (int)(blockIdx.x / P.n_chunks);
+  float x[T / WAVE];
+  load_query_row<QT, T>(P, unit, (int)threadIdx.x / WAVE, x);
   const SelUnit u = sel_unit(P, unit);
   if (chunk * kSelThreads >= u.n) return;
-  score_pages<QT, T, RT, false>(P, u, qc, qs, nullptr, first_page(chunk), P.n_chunks * kSelThreads, P.keys + (int64_t)unit * P.max_pages);
+  score_pages<QT, T, RT, false>(P, u, unit, x, qc, qs, nullptr, first_page(chunk), P.n_chunks * kSelThreads, P.keys + (int64_t)unit * P.max_pages);
 }
 template <int W>
 DEV void page_topk(const SelectParams& P) {
