@@ -555,23 +555,20 @@ DEV void select_top(const SelectParams& P, const SelUnit& u, const Keys keys, ui
     const int m = x.found[2];
     if (bits == 0) break;  // the bin is one key
     if (m > WAVE) { __syncthreads(); continue; }
-    // the m keys of the bin: the want-th largest
+    // the m keys of the bin
     for (int i = tid; i < u.n; i += W * WAVE) {
       const uint32_t k = keys[i];
       if ((k - base) >> bits == 0) x.bin_keys[atomicAdd(&x.n_bin, 1)] = k;
     }
     __syncthreads();
-    const uint32_t mine = x.bin_keys[lane];
-    int above = 0, equal = 0;
-    for (int j = 0; j < m; ++j) {
-      const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)mine, j);
-      above += o > mine;
-      equal += o == mine;
-    }
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(lane < m && above < want && above + equal >= want);
-    const int l = __builtin_ctzll(hit);
-    key = (uint32_t)__builtin_amdgcn_readlane((int)mine, l);
-    want -= __builtin_amdgcn_readlane(above, l);
+    // the largest that `want` of them reach
+    const uint32_t mine = lane < m ? x.bin_keys[lane] : 0;
+    int reach = 0;
+    for (int j = 0; j < m; j += 8)  // (lanes past the m hold 0, which no key is)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) reach += (uint32_t)readlane_i((int)mine, j + e) >= mine;
+    key = wave_max_u(lane < m && reach >= want ? mine : 0);
+    want -= __builtin_popcountll(__builtin_amdgcn_ballot_w64(mine > key));
     break;
   }
   __syncthreads();
