@@ -96,6 +96,16 @@ DEV uint32_t wave_max_u(uint32_t x) {
              max((uint32_t)readlane_i((int)x, 32), (uint32_t)readlane_i((int)x, 48)));
 }
 
+// Sum over lanes 0 .. l.
+DEV int wave_prefix_sum(int x) {
+  x += (int)dpp_u<0x111>((uint32_t)x, 0);  // row_shr 1, 2, 4, 8
+  x += (int)dpp_u<0x112>((uint32_t)x, 0);
+  x += (int)dpp_u<0x114>((uint32_t)x, 0);
+  x += (int)dpp_u<0x118>((uint32_t)x, 0);
+  const int lane = lane_id(), a = readlane_i(x, 15), b = readlane_i(x, 31), c = readlane_i(x, 47);
+  return x + (lane >= 16 ? a : 0) + (lane >= 32 ? b : 0) + (lane >= 48 ? c : 0);
+}
+
 // A float as an unsigned key of the same order (-0 as 0; not for NaN), and back.
 DEV uint32_t order_key(float x) {
   const uint32_t u = bitcast<uint32_t>(x + 0.0f);

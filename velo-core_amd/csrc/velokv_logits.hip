@@ -9,7 +9,8 @@ namespace {
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kLogitWaves = 4;
-constexpr int kList = 512;       // candidates of a wave
+constexpr int kList = 512;       // candidates of a wave, ..
+constexpr int kRoom = kList - 16;  // .. the values beside the vectors left out
 constexpr int kStepValues = 32;  // values of a thread in a step
 
 // =============================================================================
@@ -52,16 +53,28 @@ DEV uint64_t word_of(float x, int index) {
 }
 DEV int word_index(uint64_t w) { return (int)~(uint32_t)w; }
 
-// A bound that exactly k of a wave's words (N a lane, 0 = none) reach, found bit by bit;
-// 0 where there are no more than k.
+// A bound that exactly k of a wave's words (the first `used` of N a lane, 0 = none) reach,
+// found bit by bit from the first in which they differ; one that all reach where there are
+// no more than k.
 template <int N>
-DEV uint64_t kth_word(const uint64_t (&x)[N], int k) {
-  uint64_t best = 0;
-  for (int bit = 63; bit >= 0; --bit) {
+DEV uint64_t kth_word(const uint64_t (&x)[N], int k, int used) {
+  uint32_t most = 0, least = 0xFFFFFFFFu;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    most = max(most, (uint32_t)(x[i] >> 32));
+    least = min(least, x[i] ? (uint32_t)(x[i] >> 32) : 0xFFFFFFFFu);
+  }
+  most = wave_max_u(most);
+  least = ~wave_max_u(~least);
+  // (an index has at most 28 bits)
+  int bit = most > least ? 63 - __builtin_clz(most ^ least) : 27;
+  uint64_t best = ((uint64_t)most << 32 | 0xF0000000u) >> bit >> 1 << 1 << bit;
+  for (; bit >= 0; --bit) {
     const uint64_t t = best | 1ull << bit;
     int count = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[i] >= t));
+    for (int i = 0; i < N; ++i)
+      if (i < used) count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[i] >= t));
     if (count >= k) best = t;
     if (count == k) break;
   }
@@ -82,8 +95,8 @@ DEV int push_words(uint64_t* list, int n, const uint64_t (&x)[N], uint64_t least
   return n;
 }
 
-// Leaves the k largest words of the list (n > k).
-DEV int trim_list(uint64_t* list, int n, int k) {
+// Leaves the k largest words of the list (n > k), which are those that reach `least`.
+DEV int trim_list(uint64_t* list, int n, int k, uint64_t& least) {
   uint64_t x[kList / WAVE];
 #pragma unroll
   for (int i = 0; i < kList / WAVE; ++i) {
@@ -91,7 +104,7 @@ DEV int trim_list(uint64_t* list, int n, int k) {
     x[i] = at < n ? list[at] : 0;
   }
   __builtin_amdgcn_wave_barrier();
-  const uint64_t least = kth_word(x, k);
+  least = kth_word(x, k, (n + WAVE - 1) / WAVE);
   return push_words(list, 0, x, least);
 }
 
@@ -151,6 +164,7 @@ DEV void logprob_part(const LogprobParams& P) {
   constexpr int THREADS = W * WAVE;
   constexpr int GROUPS = 32 / W;            // groups of a wave's lanes
   __shared__ uint64_t lists[W][kList];
+  __shared__ u32x4 staged[W][WAVE];
   __shared__ uint64_t words[W * kMaxTop];
   __shared__ uint64_t top[kMaxTop];
   __shared__ float sums[W][3];
@@ -190,23 +204,36 @@ DEV void logprob_part(const LogprobParams& P) {
 
   const float x0 = P.n_parts == 1 && tid < P.n_tokens ? token_logit<DT>(P, row, tid) : -kInf;
   Sums s{-kInf, 0.0f, 0.0f};
-  uint64_t thr = 0;      // candidates of later steps are larger words; 0: not known
-  float thr_x = -kInf;   // its value
+  float thr_x = -kInf;   // candidates of later steps are larger
   int n = 0;             // candidates in the list
   uint64_t* list = lists[w];
-  // Adds one vector's words that can still be among the k largest of the wave's.
-  const auto take_words = [&](const uint64_t(&word)[EPV]) {
-    uint64_t most[1] = {0};
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) most[0] = max(most[0], word[e]);
-    // words that reach a bound that k lanes' largest reach: at most one in each lane but
-    // those k, so (kMaxTop - 1) EPV + 1 are the most that the list needs room for
-    const uint64_t kth = max(kth_word(most, k), thr);
-    if (n > kList - kMaxTop * EPV) n = trim_list(list, n, k);
-    n = push_words(list, n, word, kth);
-    if (kth > thr) {
-      thr = kth;
-      thr_x = key_value((uint32_t)(thr >> 32));
+  // Vector rv of every lane, 64 values at a time in the order of their indices: those above
+  // thr_x and the first `equals` that equal it. A full list is trimmed and gives a higher
+  // bound (values that equal it come later than those listed, and lose to them).
+  const auto take_vector = [&](const u32x4& rv, int v, int& equals) {
+    __builtin_amdgcn_wave_barrier();
+    staged[w][lane] = rv;
+    __builtin_amdgcn_wave_barrier();
+    const int at = (v - lane) * EPV - off, limit = v_end * EPV - off;
+#pragma unroll 1
+    for (int e = 0; e < EPV; ++e) {
+      if (n > kRoom - WAVE) {
+        uint64_t least;
+        n = trim_list(list, n, k, least);
+        thr_x = fmaxf(thr_x, key_value((uint32_t)(least >> 32)));
+        equals = 0;
+      }
+      const int index = at + e * WAVE + lane;
+      const float xv = DT == DT_F32 ? reinterpret_cast<const float*>(staged[w])[e * WAVE + lane]
+                                    : h2f(reinterpret_cast<const uint16_t*>(staged[w])[e * WAVE + lane]);
+      const bool more = index < limit && xv > thr_x;
+      const bool equal = index < limit && (thr_x == -kInf ? !more : xv == thr_x);
+      const uint64_t below = (1ull << lane) - 1, em = __builtin_amdgcn_ballot_w64(equal);
+      const bool in = more || (equal && __builtin_popcountll(em & below) < equals);
+      const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
+      if (in) list[n + __builtin_popcountll(mask & below)] = word_of(xv, index);
+      n += __builtin_popcountll(mask);
+      equals = max(0, equals - __builtin_popcountll(em));
     }
   };
   const auto step = [&](u32x4(&r)[NV], int v0, bool first) {
@@ -230,7 +257,6 @@ DEV void logprob_part(const LogprobParams& P) {
     }
     const float m = first ? fmaxf(mv, x_extra) : mv;
     if (k > 0) {
-      bool all = false;  // whether the wave looks at each vector by itself
       if (first) {
         // the maxima of 32 groups of lanes (the vectors' alone: values
         // of later steps may come before the row's last ones, which are among the extra)
@@ -258,28 +284,18 @@ DEV void logprob_part(const LogprobParams& P) {
         }
       }
       // candidates: at least thr_x in the first step, above it later
-      const bool any = first ? m >= thr_x : m > thr_x;
-      if (first && thr_x == -kInf) {
-        all = true;
-      } else if (__builtin_amdgcn_ballot_w64(any) != 0) {
-        // what the list may have to take, by vectors; where that is too much, counted
+      if (__builtin_amdgcn_ballot_w64(first || mv > thr_x) != 0) {
+        // what the list may have to take, by vectors. Where that is too much (a mask's equal
+        // values, rising ones) or no bound is known (fewer groups than n_top with a value),
+        // the vectors are taken one by one
         uint64_t hit[NV];
-        int count = first ? 2 * EPV : 0;
+        int count = n;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           hit[i] = __builtin_amdgcn_ballot_w64(first ? vm[i] >= thr_x : vm[i] > thr_x);
           count += EPV * __builtin_popcountll(hit[i]);
         }
-        if (n + count > kList) {
-          count = first ? 2 * EPV : 0;
-#pragma unroll
-          for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < EPV; ++e)
-              count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(first ? x[i][e] >= thr_x : x[i][e] > thr_x));
-        }
-        all = n + count > kList;
-        if (!all) {
+        if (count <= kRoom && !(first && thr_x == -kInf)) {
           const uint64_t below = (1ull << lane) - 1;
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
@@ -293,37 +309,25 @@ DEV void logprob_part(const LogprobParams& P) {
               n += __builtin_popcountll(mask);
             }
           }
-          if (first) {
-            const bool in = has_extra && x_extra >= thr_x;
-            const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
-            if (in) list[n + __builtin_popcountll(mask & below)] = word_of(x_extra, extra);
-            n += __builtin_popcountll(mask);
-          }
-        }
-      }
-      if (all) {
-        if (first) {
-          uint64_t word[EPV] = {};
-          word[0] = has_extra ? word_of(x_extra, extra) : 0;
-          take_words(word);
-          thr = 0;  // (the extra values are not the lowest: equal ones may still follow)
-        }
+        } else {
+          int equals = first ? k : 0;
 #pragma unroll 1
-        for (int i = 0; i < NV; ++i) {
-          u32x4 rv = r[0];
-          float most = vm[0];
+          for (int i = 0; i < NV; ++i) {
+            u32x4 rv = r[0];
 #pragma unroll
-          for (int j = 1; j < NV; ++j) { rv = i == j ? r[j] : rv; most = i == j ? vm[j] : most; }
-          if (__builtin_amdgcn_ballot_w64(thr == 0 || most > thr_x) != 0) {
-            uint64_t word[EPV];
-            const int v = v0 + i * THREADS + tid;
+            for (int j = 1; j < NV; ++j) {
+              const u32x4 o = r[j];
 #pragma unroll
-            for (int e = 0; e < EPV; ++e) word[e] = v < v_end ? word_of(value(rv, e), v * EPV - off + e) : 0;
-            take_words(word);
+              for (int d = 0; d < 4; ++d) rv[d] = i == j ? o[d] : rv[d];
+            }
+            take_vector(rv, v0 + i * THREADS + tid, equals);
+          }
+          if (n > kRoom / 2) {
+            uint64_t least;
+            n = trim_list(list, n, k, least);
+            thr_x = fmaxf(thr_x, key_value((uint32_t)(least >> 32)));
           }
         }
-      } else if (first) {
-        thr = (uint64_t)(order_key(thr_x) + 1) << 32;  // any larger value, whatever its index
       }
     }
     if (m > s.m) s = refer(s, m, c);
@@ -356,10 +360,18 @@ DEV void logprob_part(const LogprobParams& P) {
     step(a, v + STEP, false);
   }
 
+  if (k > 0 && w == 0) {  // the values beside the vectors, which have their threads in wave 0
+    static_assert(2 * EPV <= kList - kRoom && 2 * EPV <= WAVE, "room for them");
+    const bool in = has_extra && !(x_extra < thr_x);
+    const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
+    if (in) list[n + __builtin_popcountll(mask & ((1ull << lane) - 1))] = word_of(x_extra, extra);
+    n += __builtin_popcountll(mask);
+  }
   s = wave_join(s, c);
   if (lane == 0) { sums[w][0] = s.m; sums[w][1] = s.z; sums[w][2] = s.t; }
   if (k > 0) {
-    if (n > kMaxTop) n = trim_list(list, n, k);
+    uint64_t least;
+    if (n > kMaxTop) n = trim_list(list, n, k, least);
     if (lane == 0) counts[w] = n;
   }
   if (tid < k) top[tid] = 0;

@@ -479,16 +479,6 @@ DEV uint2 score_pages(const SelectParams& P, const SelUnit& u, int unit, float (
   return span;
 }
 
-// Sum over lanes 0 .. l.
-DEV int wave_prefix_sum(int x) {
-  x += (int)dpp_u<0x111>((uint32_t)x, 0);  // row_shr 1, 2, 4, 8
-  x += (int)dpp_u<0x112>((uint32_t)x, 0);
-  x += (int)dpp_u<0x114>((uint32_t)x, 0);
-  x += (int)dpp_u<0x118>((uint32_t)x, 0);
-  const int lane = lane_id(), a = readlane_i(x, 15), b = readlane_i(x, 31), c = readlane_i(x, 47);
-  return x + (lane >= 16 ? a : 0) + (lane >= 32 ? b : 0) + (lane >= 48 ? c : 0);
-}
-
 // Writes a (sequence, KV head)'s list: the kept pages and, of the scored ones, the
 // `want` with the largest keys, ties to the lower page, in ascending order. The want-th
 // largest key is found in rounds: the keys in question lie in [base, base + 2^bits);
