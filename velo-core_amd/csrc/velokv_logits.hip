@@ -53,11 +53,11 @@ DEV uint64_t word_of(float x, int index) {
 }
 DEV int word_index(uint64_t w) { return (int)~(uint32_t)w; }
 
-// A bound that exactly k of a wave's words (the first `used` of N a lane, 0 = none) reach,
+// A bound that exactly k of a wave's words (N a lane, 0 = none) reach,
 // found bit by bit from the first in which they differ; one that all reach where there are
 // no more than k.
 template <int N>
-DEV uint64_t kth_word(const uint64_t (&x)[N], int k, int used) {
+DEV uint64_t kth_word(const uint64_t (&x)[N], int k) {
   uint32_t most = 0, least = 0xFFFFFFFFu;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -73,8 +73,7 @@ DEV uint64_t kth_word(const uint64_t (&x)[N], int k, int used) {
     const uint64_t t = best | 1ull << bit;
     int count = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < used) count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[i] >= t));
+    for (int i = 0; i < N; ++i) count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[i] >= t));
     if (count >= k) best = t;
     if (count == k) break;
   }
@@ -97,6 +96,20 @@ DEV int push_words(uint64_t* list, int n, const uint64_t (&x)[N], uint64_t least
 
 // Leaves the k largest words of the list (n > k), which are those that reach `least`.
 DEV int trim_list(uint64_t* list, int n, int k, uint64_t& least) {
+  if (n <= WAVE) {  // a word a lane: its place is the number of larger ones
+    const uint64_t x = lane_id() < n ? list[lane_id()] : 0;
+    int place = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const uint64_t o = (uint64_t)(uint32_t)readlane_i((int)(x >> 32), j) << 32 | (uint32_t)readlane_i((int)x, j);
+      place += o > x;
+    }
+    const int last = __builtin_ctzll(__builtin_amdgcn_ballot_w64(place == k - 1));
+    least = (uint64_t)(uint32_t)readlane_i((int)(x >> 32), last) << 32 | (uint32_t)readlane_i((int)x, last);
+    __builtin_amdgcn_wave_barrier();
+    if (place < k) list[place] = x;
+    return k;
+  }
   uint64_t x[kList / WAVE];
 #pragma unroll
   for (int i = 0; i < kList / WAVE; ++i) {
@@ -104,7 +117,7 @@ DEV int trim_list(uint64_t* list, int n, int k, uint64_t& least) {
     x[i] = at < n ? list[at] : 0;
   }
   __builtin_amdgcn_wave_barrier();
-  least = kth_word(x, k, (n + WAVE - 1) / WAVE);
+  least = kth_word(x, k);
   return push_words(list, 0, x, least);
 }
 
@@ -146,7 +159,7 @@ DEV void rank_words(const uint64_t* words, int n, int k, uint64_t* top) {
   for (int i = (int)threadIdx.x >> 3; i < n; i += (int)blockDim.x >> 3) {
     const uint64_t x = words[i];
     int place = 0;
-#pragma unroll 2
+#pragma unroll 4
     for (int j = sub; j < n; j += 8) place += words[j] > x;
     place += (int)dpp_u<DPP_QUAD_XOR1>((uint32_t)place, 0);
     place += (int)dpp_u<DPP_QUAD_XOR2>((uint32_t)place, 0);
@@ -215,25 +228,38 @@ DEV void logprob_part(const LogprobParams& P) {
     staged[w][lane] = rv;
     __builtin_amdgcn_wave_barrier();
     const int at = (v - lane) * EPV - off, limit = v_end * EPV - off;
+    constexpr int EB = 4;  // read together
 #pragma unroll 1
-    for (int e = 0; e < EPV; ++e) {
-      if (n > kRoom - WAVE) {
+    for (int e0 = 0; e0 < EPV; e0 += EB) {
+      if (n > kRoom - EB * WAVE) {
         uint64_t least;
         n = trim_list(list, n, k, least);
         thr_x = fmaxf(thr_x, key_value((uint32_t)(least >> 32)));
         equals = 0;
       }
-      const int index = at + e * WAVE + lane;
-      const float xv = DT == DT_F32 ? reinterpret_cast<const float*>(staged[w])[e * WAVE + lane]
-                                    : h2f(reinterpret_cast<const uint16_t*>(staged[w])[e * WAVE + lane]);
-      const bool more = index < limit && xv > thr_x;
-      const bool equal = index < limit && (thr_x == -kInf ? !more : xv == thr_x);
-      const uint64_t below = (1ull << lane) - 1, em = __builtin_amdgcn_ballot_w64(equal);
-      const bool in = more || (equal && __builtin_popcountll(em & below) < equals);
-      const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
-      if (in) list[n + __builtin_popcountll(mask & below)] = word_of(xv, index);
-      n += __builtin_popcountll(mask);
-      equals = max(0, equals - __builtin_popcountll(em));
+      float xs[EB];
+#pragma unroll
+      for (int e = 0; e < EB; ++e)
+        xs[e] = DT == DT_F32 ? reinterpret_cast<const float*>(staged[w])[(e0 + e) * WAVE + lane]
+                             : h2f(reinterpret_cast<const uint16_t*>(staged[w])[(e0 + e) * WAVE + lane]);
+#pragma unroll
+      for (int e = 0; e < EB; ++e) {
+        const int index = at + (e0 + e) * WAVE + lane;
+        const bool more = index < limit && xs[e] > thr_x;
+        uint64_t mask = __builtin_amdgcn_ballot_w64(more);
+        const uint64_t below = (1ull << lane) - 1;
+        bool in = more;
+        if (equals > 0) {
+          const bool equal = index < limit && (thr_x == -kInf ? !more : xs[e] == thr_x);
+          const uint64_t em = __builtin_amdgcn_ballot_w64(equal);
+          in = more || (equal && __builtin_popcountll(em & below) < equals);
+          mask = __builtin_amdgcn_ballot_w64(in);
+          equals -= __builtin_popcountll(em);
+        }
+        if (mask == 0) continue;
+        if (in) list[n + __builtin_popcountll(mask & below)] = word_of(xs[e], index);
+        n += __builtin_popcountll(mask);
+      }
     }
   };
   const auto step = [&](u32x4(&r)[NV], int v0, bool first) {
@@ -312,7 +338,7 @@ DEV void logprob_part(const LogprobParams& P) {
         } else {
           int equals = first ? k : 0;
 #pragma unroll 1
-          for (int i = 0; i < NV; ++i) {
+          for (int i = 0; i < NV && v0 + i * THREADS + w * WAVE < v_end; ++i) {
             u32x4 rv = r[0];
 #pragma unroll
             for (int j = 1; j < NV; ++j) {
