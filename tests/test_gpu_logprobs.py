@@ -161,6 +161,31 @@ def test_alternatives_of_uneven_parts(ctx, dtype, parts):
         check(run(ctx, x, tokens, n_top), x, tokens, n_top)
 
 
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("vocab", [70, 2001, 20003])
+def test_rows_without_a_bound(ctx, dtype, vocab):
+    """Masks that leave few tokens (-infinity, the type's lowest value, zero), NaN in masked places, values in
+    order and steps; as many rows as make a row one workgroup's."""
+    r, rows = synth.rng(vocab), 1100
+    x = np.broadcast_to(r.standard_normal(vocab).astype(dtype), (rows, vocab)).copy()
+    for i, masked in enumerate((-np.inf, np.finfo(dtype).min, 0, np.nan)):
+        for j, left in enumerate((0.0, 0.01, 0.5)):
+            x[3 * i + j] = np.where(r.random(vocab) < left, r.standard_normal(vocab), masked).astype(dtype)
+    x[9:12] = np.where(np.isnan(x[9:12]), np.where(r.random((3, vocab)) < 0.5, np.nan, -np.inf), x[9:12])
+    x[12], x[13] = np.sort(x[12]), np.sort(x[13])[::-1]
+    x[14] = (np.arange(vocab) // 40).astype(dtype)
+    x[15] = -(np.arange(vocab) // 700).astype(dtype)
+    x[16] = -np.inf
+    x[16, -1] = 0
+    at, nothing = np.r_[0:18, 1099], np.r_[0, 9:12]  # rows of -infinity alone and rows with NaN: ids alone
+    usual = np.setdiff1d(at, nothing)
+    tokens = r.integers(0, vocab, (rows, 1)).astype(np.int32)
+    for n_top in (1, 5, 20, 32):
+        got = run(ctx, x, tokens, n_top)
+        assert np.array_equal(got["top_ids"][at], order(x[at], n_top))
+        check({k: v[usual] for k, v in got.items()}, x[usual], tokens[usual], n_top)
+
+
 def test_captured_calls_replay(ctx):
     """A call in parts with a workspace of its own, replayed as the logits change, beside eager calls."""
     rows, vocab, n_top = 3, 100000, 5
