@@ -785,14 +785,14 @@ DEV int sparse_qdim(int j, int g) {
   else return 32 * j + 8 * g;
 }
 
-// N query values, wherever they start.
+// N query values, wherever they start, as they are stored.
 template <int QT, int N>
-DEV void load_q(const void* q, int64_t at, float (&x)[N]) {
+struct QueryWords {
   typedef uint32_t words __attribute__((ext_vector_type(QT == DT_F32 ? N : N / 2), aligned(2)));
-  const words r = *reinterpret_cast<const words*>(reinterpret_cast<const uint8_t*>(q) + at * (QT == DT_F32 ? 4 : 2));
-#pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = QT == DT_F32 ? bitcast<float>(r[i]) : i % 2 ? half_hi(r[i / 2]) : half_lo(r[i / 2]);
-}
+  words r;
+  __device__ __forceinline__ void load(const void* q, int64_t at) { r = *reinterpret_cast<const words*>(reinterpret_cast<const uint8_t*>(q) + at * (QT == DT_F32 ? 4 : 2)); }
+  __device__ __forceinline__ float value(int i) const { return QT == DT_F32 ? bitcast<float>(r[i]) : i % 2 ? half_hi(r[i / 2]) : half_lo(r[i / 2]); }
+};
 
 template <int KV, int QT, int T, int RT>
 DEV void sparse_attn(const SparseParams& P) {
@@ -814,61 +814,29 @@ DEV void sparse_attn(const SparseParams& P) {
   const int ctx = max(0, min(P.context_lens[s], P.cap_tokens));
   const int64_t row0 = (int64_t)s * P.n_heads + (int64_t)kvh * G;
 
+  // the list's loads, then the queries', are under way before anything waits: the list's lead
+  // to the tiles
+  const int32_t* list = P.pages + (int64_t)unit * P.n_list;
+  const int first = split * P.split_entries, e1 = min(P.n_list, first + P.split_entries);
+  const int ahead = list[min(first + lane, e1 - 1)];
   // q^T: row n of each 16-row tile (rows past the group repeat its last one: their columns of
   // the results are not used), zeros past head_dim
-  half8 qa[RT][F32 ? 1 : KC], qlo[RT][QSPLIT ? KC : 1];
-  float qf[RT][F32 ? T / 4 : 1], scale_log2[RT];
+  constexpr int QN = F32 ? 4 : 8, QC = F32 ? T / 16 : KC;  // values of a chunk, chunks
+  const auto qdim = [&](int j) { return F32 ? 16 * j + 4 * g : sparse_qdim<KV, T>(j, g); };
+  QueryWords<QT, QN> qw[RT][QC];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    scale_log2[rt] = P.scale_log2;
-    const int64_t off = (row0 + min(16 * rt + n, G - 1)) * P.io_hd;
-    if constexpr (F32) {
+  for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int j = 0; j < T / 16; ++j) {
-        const int d = 16 * j + 4 * g;
-        float x[4];
-        load_q<QT, 4>(P.q, off + min(d, P.io_hd - 4), x);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) qf[rt][4 * j + e] = d < P.io_hd ? x[e] : 0.0f;
-      }
-    } else {
-      float x[KC][8], top = 0.0f;
-#pragma unroll
-      for (int j = 0; j < KC; ++j) {
-        const int d = sparse_qdim<KV, T>(j, g);
-        load_q<QT, 8>(P.q, off + min(d, P.io_hd - 8), x[j]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[j][i] = d < P.io_hd ? x[j][i] : 0.0f;
-          if constexpr (QSPLIT) top = fmaxf(top, fabsf(x[j][i]));
-        }
-      }
-      int up = 0;  // an fp32 row is taken times 2^up, which brings its largest to [2^13, 2^14): fp16 ends at 2^16
-      if constexpr (QSPLIT) {
-        top = fmaxf(top, shfl_xor(top, 16));
-        top = fmaxf(top, shfl_xor(top, 32));
-        up = top > 0.0f && top < kInf ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
-        scale_log2[rt] = __builtin_amdgcn_ldexpf(P.scale_log2, -up);
-      }
-#pragma unroll
-      for (int j = 0; j < KC; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float v = QSPLIT ? __builtin_amdgcn_ldexpf(x[j][i], up) : x[j][i];
-          qa[rt][j][i] = (_Float16)v;
-          if constexpr (QSPLIT) qlo[rt][j][i] = (_Float16)(v - (float)qa[rt][j][i]);
-        }
-    }
-  }
+    for (int j = 0; j < QC; ++j)
+      qw[rt][j].load(P.q, (row0 + min(16 * rt + n, G - 1)) * P.io_hd + min(qdim(j), P.io_hd - QN));
 
   if (w == 0) {  // the part's entries that name a page of the context
     const int32_t* bt = P.block_tables + (int64_t)table_row(P.seq_rows, s, P.bt_rows) * P.bt_stride;
-    const int32_t* list = P.pages + (int64_t)unit * P.n_list;
-    const int e1 = min(P.n_list, (split + 1) * P.split_entries), ptok = 16 * P.page_tiles;
+    const int ptok = 16 * P.page_tiles;
     int count = 0;
     bool bad = false;
-    for (int e0 = split * P.split_entries; e0 < e1; e0 += WAVE) {
-      const int col = e0 + lane < e1 ? list[e0 + lane] : -1;
+    for (int e0 = first; e0 < e1; e0 += WAVE) {
+      const int col = e0 + lane < e1 ? (e0 == first ? ahead : list[e0 + lane]) : -1;
       const bool in = col >= 0 && (int64_t)col * ptok < ctx;
       const int raw = in ? bt[col] : 0;
       bad |= raw < 0 || raw >= P.n_pages;
@@ -882,6 +850,40 @@ DEV void sparse_attn(const SparseParams& P) {
     }
     if (lane == 0) n_valid = count;
     if (__builtin_amdgcn_ballot_w64(bad) != 0 && lane == 0) flag_misuse(P.err, MISUSE_PAGE_OUT_OF_POOL);
+  }
+
+  half8 qa[RT][F32 ? 1 : KC], qlo[RT][QSPLIT ? KC : 1];
+  float qf[RT][F32 ? T / 4 : 1], scale_log2[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    scale_log2[rt] = P.scale_log2;
+    float top = 0.0f;
+    if constexpr (QSPLIT) {
+#pragma unroll
+      for (int j = 0; j < QC; ++j)
+#pragma unroll
+        for (int i = 0; i < QN; ++i) top = fmaxf(top, qdim(j) < P.io_hd ? fabsf(qw[rt][j].value(i)) : 0.0f);
+    }
+    int up = 0;  // an fp32 row is taken times 2^up, which brings its largest to [2^13, 2^14): fp16 ends at 2^16
+    if constexpr (QSPLIT) {
+      top = fmaxf(top, shfl_xor(top, 16));
+      top = fmaxf(top, shfl_xor(top, 32));
+      up = top > 0.0f && top < kInf ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+      scale_log2[rt] = __builtin_amdgcn_ldexpf(P.scale_log2, -up);
+    }
+#pragma unroll
+    for (int j = 0; j < QC; ++j)
+#pragma unroll
+      for (int i = 0; i < QN; ++i) {
+        const float x = qdim(j) < P.io_hd ? qw[rt][j].value(i) : 0.0f;
+        if constexpr (F32) {
+          qf[rt][QN * j + i] = x;
+        } else {
+          const float v = QSPLIT ? __builtin_amdgcn_ldexpf(x, up) : x;
+          qa[rt][j][i] = (_Float16)v;
+          if constexpr (QSPLIT) qlo[rt][j][i] = (_Float16)(v - (float)qa[rt][j][i]);
+        }
+      }
   }
   __syncthreads();
   const int n_tiles = __builtin_amdgcn_readfirstlane(n_valid) * P.page_tiles;
