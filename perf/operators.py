@@ -407,9 +407,10 @@ def _own_cache(st):
     st.update(ctx=ctx, pool=pool)
     if case["kind"] != "attend":
         st["index"] = velokv.KeyIndex(ctx, pool)
+    if case["kind"] in ("select", "both"):  # the index that earlier steps left
         ctx.index_update(st["index"], 0, **rows)
         torch.cuda.synchronize()
-    if case["kind"] == "index":
+    if case["kind"] == "index":  # no bounds yet: what the case reads back is what its update wrote
         n = len(st["touched"])
         st["lower"] = torch.empty((n, case["kv_heads"], case["dim"]), device="cuda")
         st["upper"] = torch.empty_like(st["lower"])
