@@ -103,8 +103,9 @@ typedef struct vk_block_manager vk_block_manager;
 const char* vk_last_error(void);
 
 /* Open `device`, load the gfx950 code object (NULL = velokv_gfx950.co next to
- * this library; the code objects of sparse decode and of the log probabilities
- * are always those next to it) and resolve every kernel.
+ * this library) and resolve every kernel. The code objects of sparse decode and of
+ * the log probabilities are always those next to the library; without one of them
+ * the calls that run its kernels fail with VK_ERR_NOT_WIRED, and no others.
  * Replaces MetalMemoryRuntime::new's device/queue/library setup
  * (metal/runtime.rs:141-186) and load_metal_library (metal/runtime.rs:29-60). */
 int vk_ctx_create(int device, const char* code_object_path, vk_ctx** out);

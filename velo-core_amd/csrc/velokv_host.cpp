@@ -204,6 +204,18 @@ int load_object(vk_ctx* ctx, const std::string& path, const std::vector<std::str
   return VK_OK;
 }
 
+// Loads a code object beside this library that only some calls need. Without it the context
+// has the other kernels, and a launch of one of these says why it is refused.
+void load_beside(vk_ctx* ctx, const char* file, const std::vector<std::string>& names) {
+  if (load_object(ctx, beside_library(file), names) == VK_OK) return;
+  (void)hipGetLastError();  // the refused load is no error of a later call
+  for (const auto& nm : names) {
+    ctx->fns.erase(nm);
+    ctx->max_threads.erase(nm);
+    ctx->unloaded[nm] = g_last_error;
+  }
+}
+
 // Unloads a context's code objects and deletes it.
 void unload(vk_ctx* ctx) {
   for (hipModule_t m : ctx->modules) hipModuleUnload(m);
@@ -277,12 +289,12 @@ extern "C" int vk_ctx_create(int device, const char* code_object_path, vk_ctx** 
         for (int qt = 0; qt < 2; ++qt) names.push_back(tree_pfx_name(kv, g, qt));
     }
   int rc = load_object(ctx, code_object_path ? std::string(code_object_path) : beside_library("velokv_gfx950.co"), names);
-  if (!rc) rc = load_object(ctx, beside_library("velokv_sparse_gfx950.co"), sparse_kernel_names());
-  if (!rc) rc = load_object(ctx, beside_library("velokv_logits_gfx950.co"), logits_kernel_names());
   if (rc) {
     unload(ctx);
     return rc;
   }
+  load_beside(ctx, "velokv_sparse_gfx950.co", sparse_kernel_names());
+  load_beside(ctx, "velokv_logits_gfx950.co", logits_kernel_names());
   e = hipMalloc(reinterpret_cast<void**>(&ctx->err_word), 256);
   if (e == hipSuccess) e = hipMemset(ctx->err_word, 0, 256);
   if (e != hipSuccess) {

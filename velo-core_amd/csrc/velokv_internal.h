@@ -35,6 +35,7 @@ struct vk_ctx {
   // once at vk_ctx_create: a launch with more faults the device, so launch()
   // refuses it
   std::unordered_map<std::string, int> max_threads;
+  std::unordered_map<std::string, std::string> unloaded;  // kernels of a code object that did not load: why
   std::mutex ws_mu;
   void* ws = nullptr;
   uint64_t ws_bytes = 0;
@@ -84,11 +85,18 @@ inline int set_device(const vk_ctx* ctx) {
   return VK_OK;
 }
 
+// A kernel that the context does not have.
+inline int no_kernel(const vk_ctx* ctx, const char* name) {
+  auto it = ctx->unloaded.find(name);
+  if (it != ctx->unloaded.end()) return fail(VK_ERR_NOT_WIRED, "kernel %s: %s", name, it->second.c_str());
+  return fail(VK_ERR_NOT_WIRED, "kernel %s is not in the code object", name);
+}
+
 // A workgroup shape the kernel was compiled for: at least one thread and at most
 // its __launch_bounds__ (HIP_FUNC_ATTRIBUTE_MAX_THREADS_PER_BLOCK).
 inline int check_launch_shape(const vk_ctx* ctx, const char* name, uint64_t threads) {
   auto it = ctx->max_threads.find(name);
-  if (it == ctx->max_threads.end()) return fail(VK_ERR_NOT_WIRED, "kernel %s is not in the code object", name);
+  if (it == ctx->max_threads.end()) return no_kernel(ctx, name);
   if (threads == 0 || threads > (uint64_t)it->second)
     return fail(VK_ERR_BAD_ARG, "kernel %s launched with %llu threads per workgroup; it was compiled for at most %d",
                 name, (unsigned long long)threads, it->second);
@@ -98,7 +106,7 @@ inline int check_launch_shape(const vk_ctx* ctx, const char* name, uint64_t thre
 template <typename P>
 int launch(const vk_ctx* ctx, const char* name, dim3 grid, dim3 block, const P& params, void* stream) {
   hipFunction_t f = ctx->fn(name);
-  if (!f) return fail(VK_ERR_NOT_WIRED, "kernel %s is not in the code object", name);
+  if (!f) return no_kernel(ctx, name);
   int rc = check_launch_shape(ctx, name, (uint64_t)block.x * block.y * block.z);
   if (rc) return rc;
   void* args[] = {const_cast<P*>(&params)};
