@@ -592,7 +592,8 @@ typedef struct vk_logprob_args {
   int64_t row_stride;         /* elements from a row to the next; 0 = vocab     */
   int32_t n_rows;
   int32_t vocab;              /* up to 2^28                                     */
-  float scale;                /* x = scale * logit (1 / temperature); 0 = 1     */
+  float scale;                /* x = scale * logit (1 / temperature); 0 = 1; up to 2.35e38
+                                 (scale * log2(e) is finite in fp32)            */
   const int32_t* tokens;      /* dev [n_rows][n_tokens] given tokens            */
   int32_t n_tokens;           /* 0 = none                                       */
   float* token_logprobs;      /* dev [n_rows][n_tokens]                         */

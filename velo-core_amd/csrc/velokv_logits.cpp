@@ -25,7 +25,9 @@ int plan_logprobs(const vk_ctx* ctx, const vk_logprob_args* a, LogprobPlan* pl) 
   if (a->vocab > kMaxVocab) return fail(VK_ERR_UNSUPPORTED, "vocabulary of %d (up to %d)", a->vocab, kMaxVocab);
   if (a->n_top > kMaxTop) return fail(VK_ERR_UNSUPPORTED, "n_top %d (up to %d)", a->n_top, kMaxTop);
   if (a->n_top > a->vocab) return fail(VK_ERR_BAD_ARG, "n_top %d exceeds the vocabulary (%d)", a->n_top, a->vocab);
-  if (!(a->scale >= 0.f) || std::isinf(a->scale)) return fail(VK_ERR_BAD_ARG, "scale must be finite and not negative");
+  // the kernels' exponents are (x - max) * scale * log2(e), whose factor has to be finite (0 at the maximum)
+  if (!(a->scale >= 0.f) || !std::isfinite(a->scale * 1.4426950408889634f))
+    return fail(VK_ERR_BAD_ARG, "scale must not be negative, and finite times log2(e)");
   // Parts of 8192 values (a step of a workgroup of four waves) at least, about four
   // workgroups a CU (64 rows of 128000: 18.2 us, 21.4 with two a CU, 22.9 with one of 16
   // waves a row); rows of 2 to 4 steps, no more than the CUs, take one workgroup of 16 waves
