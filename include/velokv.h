@@ -535,7 +535,7 @@ typedef struct vk_sparse_args {
   int32_t* pages;             /* dev [S][n_kv_heads][n_pages]: places in the sequence's
                                  table row (0 = its first page); written by the selection,
                                  read by the attention                          */
-  int32_t n_pages;            /* length of a list                              */
+  int32_t n_pages;            /* length of a list, 1..2^30                     */
   int32_t n_first;            /* selection: the first n_first and the last n_last pages of a */
   int32_t n_last;             /* context are always listed; n_first + n_last <= n_pages */
   const int32_t* block_tables;/* dev [rows][bt_stride]; NULL = the pool's slot table */

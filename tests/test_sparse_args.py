@@ -49,3 +49,13 @@ def test_scale_of_logits(ask):
     for bad in (first, np.finfo(np.float32).max, np.inf, np.nan, -1.0):
         rc, _, message = ask("scale", repr(float(bad)))
         assert rc == velokv.ERR_BAD_ARG and "scale" in message, bad
+
+
+def test_length_of_a_list(ask):
+    """The kernels count a list's entries in 32 bits and step past its end by up to a workgroup: indices of a
+    list near 2^31 entries would wrap to before its start."""
+    for n in (1, 512, 1 << 20, 1 << 30):
+        assert ask("list", n, 0, 1000)[0] == _capi.OK, n
+    for n in ((1 << 30) + 1, 2 ** 31 - 513, 2 ** 31 - 512, 2 ** 31 - 1):
+        rc, _, message = ask("list", n, 1, 1000)
+        assert rc == velokv.ERR_UNSUPPORTED and str(n) in message, n

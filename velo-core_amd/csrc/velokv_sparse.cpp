@@ -20,6 +20,8 @@ struct vk_key_index {
 namespace {
 
 constexpr int kMaxGroup = 32;  // two 16-row matrix-core tiles
+// The kernels hold an entry's place in an int, up to a workgroup past the list's end
+constexpr int kMaxList = 1 << 30;
 // HIP takes less than 2^32 threads in a grid
 constexpr uint64_t kMaxThreads = (1ull << 32) - 1;
 
@@ -78,6 +80,7 @@ int plan_sparse(const vk_ctx* ctx, const vk_pool* pool, const vk_sparse_args* a,
   if (pl->group > kMaxGroup) return fail(VK_ERR_UNSUPPORTED, "GQA group size %d (sparse decode supports up to %d)", pl->group, kMaxGroup);
   if (a->q_dtype != VK_DT_F32 && a->q_dtype != VK_DT_F16) return fail(VK_ERR_BAD_ARG, "q_dtype %d", a->q_dtype);
   if (a->n_pages <= 0) return fail(VK_ERR_BAD_ARG, "n_pages must be positive");
+  if (a->n_pages > kMaxList) return fail(VK_ERR_UNSUPPORTED, "a list of %d pages (up to %d)", a->n_pages, kMaxList);
   if (a->n_first < 0 || a->n_last < 0 || (int64_t)a->n_first + a->n_last > a->n_pages)
     return fail(VK_ERR_BAD_ARG, "n_first %d and n_last %d do not fit a list of %d pages", a->n_first, a->n_last, a->n_pages);
   if (int rc = resolve_table(pool, a->block_tables, a->bt_stride, a->max_context_len, &pl->table)) return rc;
