@@ -300,7 +300,7 @@ DEV SelUnit sel_unit(const SelectParams& P, int unit) {
   u.kvh = unit % P.n_kv_heads;
   u.s = unit / P.n_kv_heads;
   const int ctx = max(0, min(P.context_lens[u.s], P.cap_tokens));
-  u.np = (ctx + P.page_tokens - 1) / P.page_tokens;
+  u.np = (int)(((uint32_t)ctx + (uint32_t)P.page_tokens - 1) / (uint32_t)P.page_tokens);  // ctx ends at 2^31 - 1
   u.lo = P.n_first;
   u.n = u.np > P.n_list ? u.np - P.n_first - P.n_last : 0;  // none: all pages are listed
   u.bt = P.block_tables + (int64_t)table_row(P.seq_rows, u.s, P.bt_rows) * P.bt_stride;
