@@ -74,13 +74,17 @@ class SpeculativeTree:
     def verify_logits(self, ctx, logits, dtype: int, vocab: int, row_stride: int = 0, stream=None) -> TreeVerifyResult:
         """The target model's most probable token after each node, and its log probability, from device logits
         [n_nodes][row_stride] (vk_token_logprobs): what find_best_path and best_path_nodes take
-        (verify_tree, speculative.rs:217-242). Waits for the stream."""
+        (verify_tree, speculative.rs:217-242). Waits for the stream. The scratch is the call's own, so trees may be
+        verified on several streams at once."""
         n = len(self.nodes)
-        ids, top = ctx.alloc(4 * n), ctx.alloc(4 * n)
-        ctx.token_logprobs(logits, dtype, n, vocab, top_ids=ids, top_logprobs=top, n_top=1, row_stride=row_stride,
-                           stream=stream)
+        scratch = -(-ctx.token_logprobs_workspace_bytes(n, vocab, 1, dtype) // 16) * 16
+        buf = ctx.alloc(scratch + 8 * n)  # scratch, ids, log probabilities
+        ids = buf.ptr + scratch
+        ctx.token_logprobs(logits, dtype, n, vocab, top_ids=ids, top_logprobs=ids + 4 * n, n_top=1, row_stride=row_stride,
+                           workspace=buf, workspace_bytes=scratch, stream=stream)
         ctx.sync(stream)
-        return TreeVerifyResult(ids.download((n,), np.int32).tolist(), top.download((n,), np.float32).tolist())
+        got = buf.download((2, n), np.int32, scratch)
+        return TreeVerifyResult(got[0].tolist(), got[1].view(np.float32).tolist())
 
     def path_nodes(self, node_idx: int) -> list[int]:
         """Node indices from the root to node_idx (get_path, speculative.rs:81-94, as node indices)."""
