@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import enum
+import weakref
 from collections import deque
 from dataclasses import dataclass
 
@@ -485,6 +486,7 @@ class Pool:
         h = C.c_void_p()
         check(lib().vk_pool_create(ctx.h, C.byref(d), C.byref(h)))
         self.h = h
+        self._indexes = weakref.WeakSet()  # KeyIndex objects of this pool, which do not outlive it
         out = _capi.PoolDesc()
         check(lib().vk_pool_get_desc(self.h, C.byref(out)))
         self.desc = out
@@ -492,7 +494,10 @@ class Pool:
         self.n_kv_heads, self.head_dim, self.kv_type = n_kv_heads, head_dim, kv_type
 
     def close(self):
+        """Frees the pool and its key indexes."""
         if self.h:
+            for index in list(self._indexes):
+                index.close()
             lib().vk_pool_destroy(self.h)
             self.h = C.c_void_p()
 
@@ -576,13 +581,14 @@ class Pool:
 
 
 class KeyIndex:
-    """Bounds of the keys of every page of a pool (vk_index_create), for select_pages."""
+    """Bounds of the keys of every page of a pool (vk_index_create), for select_pages. Closed with its pool."""
 
     def __init__(self, ctx: Context, pool: Pool):
-        self.ctx, self.pool = ctx, pool  # the pool outlives its index
+        self.ctx, self.pool = ctx, pool
         h = C.c_void_p()
         self.h = h
         check(lib().vk_index_create(ctx.h, pool.h, C.byref(h)))
+        pool._indexes.add(self)
 
     def close(self):
         if self.h:
