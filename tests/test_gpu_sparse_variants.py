@@ -130,6 +130,61 @@ def test_slot_table(ctx, kv, page):
     assert e.value.code == velokv.ERR_BAD_ARG
 
 
+@pytest.mark.parametrize("page,head_dim,group", [(256, 8, 2), (144, 120, 5), (16, 72, 17)])
+@pytest.mark.parametrize("q_dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("kv", KVS)
+def test_a_layer_among_others(ctx, kv, q_dtype, page, head_dim, group):
+    """Layer 2 of 3, three KV heads, the longest pages and the least head_dim, queries and results that start one
+    element into their buffers, and table entries past a context that name nothing."""
+    c = Cache(ctx, kv, [page * 12 + 5, 3, page * 7], n_kv_heads=3, head_dim=head_dim, page=page, seed=44)
+    pool = velokv.Pool(ctx, 3, c.n_pages, page, 3, head_dim, kv)
+    pool.upload_layer(2, c.pool.download_layer(0))
+    for s, n in enumerate(c.lens):
+        c.table[s, -(-int(n) // page):] = 2 ** 31 - 1
+    one, index, q = velokv.KeyIndex(ctx, c.pool), velokv.KeyIndex(ctx, pool), queries(c, 3, 3 * group, q_dtype)
+    ctx.index_update(one, 0, **c.dev())
+    for layer in (2, 1):  # the layer beside it, of zeros, is not its own
+        ctx.index_update(index, layer, **c.dev())
+    shifted, out = ctx.upload(np.r_[q.reshape(-1)[:1], q.reshape(-1)]), ctx.upload(np.full(q.size + 2, np.nan, np.float32))
+    lists = ctx.upload(np.full((3, 3, 4), 77, np.int32))
+    ctx.select_decode(index, 2, shifted.ptr + q.itemsize, dt(q), out.ptr + 4, lists, 4, n_heads=q.shape[1], **c.dev())
+    ctx.sync()  # and no page is reported
+    lists, out = lists.download((3, 3, 4), np.int32), out.download()
+    assert np.array_equal(lists, select(c, one, q, c.lens, [0, 1, 2], 4))
+    assert np.isnan(out[0]) and np.isnan(out[-1])
+    got = out[1:-1].reshape(q.shape)
+    assert np.array_equal(got, sparse(c, q, lists, c.lens, [0, 1, 2]))
+    close(got, attend(c, q, lists, c.lens, [0, 1, 2]))
+
+
+@pytest.mark.parametrize("size", [2.0 ** -30, 2.0 ** -66])
+def test_small_value_scales(ctx, size):
+    """int8 values of fp32 scales down to 2^-74 keep their precision."""
+    c = Cache(ctx, O.I8_REF, [16 * 24], seed=45)
+    r = synth.rng(46)
+    k = r.standard_normal((16 * 24, c.hkv, c.hd)).astype(np.float32)
+    v = (r.standard_normal(k.shape) * size).astype(np.float32)
+    slots = synth.slots_for_positions(c.table, np.arange(16 * 24), 16, np.zeros(16 * 24, int))
+    ctx.append(c.pool, 0, ctx.upload(k), ctx.upload(v), velokv.DT_F32, ctx.upload(slots), len(k))
+    c.read()
+    lists = np.broadcast_to(np.arange(24, dtype=np.int32), (1, 2, 24))
+    q = queries(c, 1, 8, np.float16)
+    close(sparse(c, q, lists, c.lens, [0]), attend(c, q, lists, c.lens, [0]))
+
+
+def test_subnormal_keys_and_values(ctx):
+    """fp16 keys and values below 2^-14 keep the bits they have."""
+    c = Cache(ctx, O.F16, [16 * 24 - 3], seed=47)
+    r = synth.rng(48)
+    k, v = ((r.standard_normal((16 * 24 - 3, c.hkv, c.hd)) * 2.0 ** -17).astype(np.float16) for _ in range(2))
+    c.append(0, np.arange(len(k)), k, v)
+    c.read()
+    lists = np.broadcast_to(np.arange(24, dtype=np.int32), (1, 2, 24))
+    for q_dtype in (np.float16, np.float32):
+        q = queries(c, 1, 8, q_dtype)
+        close(sparse(c, q, lists, c.lens, [0], scale=2.0 ** 14), attend(c, q, lists, c.lens, [0], 2.0 ** 14))
+
+
 def test_index_of_a_closed_pool(ctx):
     """The pool's close closes its indexes; calls on them are refused."""
     pool = velokv.Pool(ctx, 1, 4, 16, 1, 64, velokv.KV_F16)
