@@ -489,9 +489,11 @@ int vk_tree_verify(vk_ctx* ctx, vk_pool* pool, const vk_tree_args* a, void* stre
  * Attention of a decode step over a few pages of a long context, chosen for each
  * query by a cheap score. No counterpart in the reference, whose kernels read the
  * whole context (kernels.metal:440-501). A key index holds, for every layer, page
- * and KV head, the lower and upper bound of the page's keys in each dim, as int8
- * codes with one fp32 scale: 2 * head_dim + 4 bytes (head_dim rounded up to 64 or
- * 128) beside a page's block_size * head_dim elements of K. A decode step appends
+ * and KV head, the least and the largest of the page's keys in each dim (its bounds),
+ * each as the nearest int8 code, with one fp32 scale: 2 * head_dim + 4 bytes (head_dim
+ * rounded up to 64 or 128) beside a page's block_size * head_dim elements of K. A code
+ * is off by up to half a step, to either side: the score made of codes estimates the
+ * page's largest q . k, it does not bound it. A decode step appends
  * its tokens (vk_append_rope), brings the index up to date (vk_index_update), and
  * chooses and attends (vk_select_decode). */
 typedef struct vk_key_index vk_key_index;
@@ -575,7 +577,8 @@ int vk_select_pages(vk_ctx* ctx, vk_key_index* index, const vk_sparse_args* a, v
  * past the context name nothing; a page listed twice counts twice; rows with no
  * token are 0. a->n_first and a->n_last are checked, not used. Results are those of
  * fp32 arithmetic over the stored values to about 2^-20 of the largest, whatever the
- * types. With a query or a listed key that is not finite the row is unspecified (in
+ * types (value scales of VK_KV_I8_REF from 2^-80 on; below, precision falls with them).
+ * With a query or a listed key that is not finite the row is unspecified (in
  * bounds, no other row is affected); so is the dim of a listed value that is not. */
 int vk_sparse_decode(vk_ctx* ctx, vk_pool* pool, const vk_sparse_args* a, void* stream);
 
@@ -609,8 +612,8 @@ typedef struct vk_logprob_args {
  * in fp32. A logit of -infinity has probability 0; a row of nothing else has log
  * probabilities of -infinity, the entropy 0 and the lowest ids on top. A row with NaN
  * or +infinity has NaN log probabilities and entropy (NaN counts as -infinity in the
- * choice of top_ids). A given token outside the vocabulary has -infinity. Reads the
- * logits once. */
+ * choice of top_ids). A given token outside the vocabulary has -infinity (NaN in such a
+ * row). Reads the logits once. */
 int vk_token_logprobs(vk_ctx* ctx, const vk_logprob_args* a, void* stream);
 int vk_token_logprobs_workspace(const vk_ctx* ctx, const vk_logprob_args* a, uint64_t* bytes);
 

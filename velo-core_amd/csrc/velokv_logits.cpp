@@ -29,9 +29,11 @@ int plan_logprobs(const vk_ctx* ctx, const vk_logprob_args* a, LogprobPlan* pl) 
   if (!(a->scale >= 0.f) || !std::isfinite(a->scale * 1.4426950408889634f))
     return fail(VK_ERR_BAD_ARG, "scale must not be negative, and finite times log2(e)");
   // Parts of 8192 values (a step of a workgroup of four waves) at least, about four
-  // workgroups a CU (64 rows of 128000: 18.2 us, 21.4 with two a CU, 22.9 with one of 16
-  // waves a row); rows of 2 to 4 steps, no more than the CUs, take one workgroup of 16 waves
-  // each and no join (one of 32000 fp32: 9.3 us, 11.5 in parts).
+  // workgroups a CU (64 rows of 128000 fp16, 20 alternatives: 14.9 us, 16.7 with two a CU, 19.7
+  // with one of 16 waves a row; one row: 8.7, 16.8 with 16 waves). Rows of 2 to 4 steps, no more
+  // than the CUs, take one workgroup of 16 waves each and no join (256 of 32000 fp16: 9.2 us, 12.1
+  // in parts; 256 of 20000 with 20 alternatives: 9.7, 14.9; 128 of 20000 fp32: 9.7, 10.5; one of
+  // 32000 fp32: 8.6 either way; 64 of 32000 fp32: 10.0, 9.5).
   constexpr int kStep = 8192;
   const int64_t rows = std::max<int64_t>(1, a->n_rows);
   const int64_t steps = ((int64_t)a->vocab + kStep - 1) / kStep;

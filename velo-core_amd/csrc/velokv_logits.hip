@@ -27,14 +27,15 @@ constexpr int kStepValues = 32;  // values of a thread in a step
 // it, are candidates. Where they may not fit the list (many equal values, rising ones) or
 // fewer groups than n_top have a value (rows that a mask leaves little of, short rows), a
 // wave takes its vectors one by one through LDS, the bound's equals up to n_top of them, and
-// trims a full list (60 rows, one in eight masked to 1 % of 16000 fp32 values: 9.8 us with 5
-// alternatives and 22 with 32).
+// trims a full list (60 rows, one in eight masked to 1 % of 20000 fp32 values: 9.3 us with 5
+// alternatives, 10.9 with 31 and 22 with 32).
 //
-// Bound: 1500 rows of 50001 fp16: 35 us, 150 MB at 4.3 TB/s, by the vector ALUs' work (ten
-// instructions a value) beside the loads. 64 rows of 128000 fp16: 14.5 us from the last-level
-// cache and 20 from HBM, of them 9.3 without alternatives; every wave has one step, so its
-// loads and its work do not overlap, and the join is a launch of its own (4.3 us). One row:
-// launch and latency (32000 fp32: 8.6 us). The exponent of base 2 is also the entropy's
+// Bound: 1500 rows of 50001 fp16: 35 us, 150 MB at 4.3 TB/s (31 without alternatives), by the
+// vector ALUs' work (ten instructions a value) beside the loads. 64 rows of 128000 fp16 with
+// 20 alternatives: 14.5 us from the last-level cache and 15.0 from HBM, 8.6 without
+// alternatives; every wave has one step, so its loads and its work do not overlap, and the
+// join is a launch of its own (4.4 us). One row: launch and latency (32000 fp32: 8.5 us, 9.5
+// from HBM). The exponent of base 2 is also the entropy's
 // factor, which saves a product a value.
 // =============================================================================
 struct Sums { float m, z, t; };

@@ -244,7 +244,7 @@ struct IndexUpdateParams {
   const int32_t* first_tokens;  // [S] first new position, or null: 0
   const int32_t* context_lens;
   uint32_t* err;
-  uint32_t tile_bytes, stile_bytes, s_step;
+  uint32_t tile_bytes, stile_bytes;
   int32_t bt_stride, bt_rows, n_seqs, n_kv_heads, n_pages, page_tiles;
   int32_t max_pages;        // pages of a sequence in the grid
   int32_t seq_wgs;          // workgroups of a sequence
@@ -310,7 +310,7 @@ struct LogprobParams {
   float* entropy;           // [n_rows] or null
   int32_t* top_ids;         // [n_rows][n_top]
   float* top_logprobs;      // [n_rows][n_top]
-  float* part_sums;         // [n_rows][n_parts][4]: max, sum of e^(x - max), sum of e^(x - max) (x - max)
+  float* part_sums;         // [n_rows][n_parts][4]: m = max x, sum of 2^e, sum of 2^e e, e = (x - m) scale log2(e)
   uint64_t* part_top;       // [n_rows][n_parts][n_top], largest first
   int64_t row_stride;
   int32_t n_rows, vocab, n_tokens, n_top, n_parts, part_len;

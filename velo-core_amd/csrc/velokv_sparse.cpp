@@ -87,9 +87,11 @@ int plan_sparse(const vk_ctx* ctx, const vk_pool* pool, const vk_sparse_args* a,
   pl->units = (uint64_t)a->n_seqs * d.n_kv_heads;
   pl->max_pages = (int)(((int64_t)a->max_context_len + d.block_size - 1) / d.block_size);
   const int64_t units = std::max<int64_t>(1, (int64_t)pl->units);
-  // selection: one workgroup per (sequence, KV head), or several and a second launch, which
-  // takes longer than 2048 pages of a CU do (8 heads of 8125 pages: 72 us in one launch, 21.6
-  // in two)
+  // selection: one workgroup per (sequence, KV head), or several and a second launch past 2048
+  // pages of few of them. One launch against two, us: 8 of 1024 pages 9.3 and 11.8, of 2048 13.9
+  // and 12.8, of 4096 22.4 and 15.0, of 8125 38.8 and 19.6; 32 of 2560 17.2 and 14.0, of 8125
+  // 48.2 and 27.2; 128 of 2560 22.5 and 28.1, of 8125 70.6 and 62.1. Between the two (64 of 4096:
+  // 28.2 and 22.1, of 8125: 50.4 and 38.0) the rule takes the slower
   pl->n_chunks = 0;
   pl->select_bytes = 0;
   if (pl->max_pages > kSelPages || (pl->max_pages > 2048 && 8 * units <= ctx->n_cu)) {
@@ -99,10 +101,10 @@ int plan_sparse(const vk_ctx* ctx, const vk_pool* pool, const vk_sparse_args* a,
   }
   // attention: eight waves a CU (more do not fit beside their registers), in one workgroup
   // per (sequence, KV head) where there are as many as CUs, in parts of the list else. Two of
-  // four waves a CU where there are twice as many (512 fp16: 45.6 us, 48.6 with eight waves
-  // each; 256 int8: 30.2 with eight, 34.6 with four). At most a part a CU (64 of up to 50
-  // pages, fp32: 18.0 us, 22.5 with two), of a tile a wave at least (32 of 64 pages: 11.5 us,
-  // 12.9 with two tiles)
+  // four waves a CU where there are twice as many (512 fp16: 43.9 us, 46.7 with eight waves
+  // each; 256 int8: 26.2 with eight, 26.5 with four). At most a part a CU (64 of up to 50
+  // pages, fp32: 17.8 us, 23.6 with two), of a tile a wave at least (32 of 64 pages: 10.0 us,
+  // 11.9 with two tiles)
   const int pt = pool->geom.page_tiles, cus = ctx->n_cu;
   pl->waves = units >= 2 * cus || pl->group > 16 ? 4 : 8;
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(cus / units, (int64_t)a->n_pages * pt / 8));

@@ -31,10 +31,11 @@ DEV int to_code(float x, float inv) { return (int)fminf(fmaxf(rintf(x * inv), -1
 // with one fp32 scale top / 127, top = max_d max(|lo|, |hi|). One wave per (page,
 // KV head): lanes take 16-byte chunks of the K tiles, so each holds the bounds of a
 // fixed set of dims and the tokens' lanes are joined by lane exchanges at the end.
-// A page with a key that is not finite has the scale infinity (it is chosen before
-// any other).
+// A code is the nearest, so a bound may lie up to half a step (top / 254) inside the
+// keys' range. A page with a key that is not finite has the scale infinity (it is chosen
+// before any other).
 // Bound: the chain of table, keys and codes. The newest pages of 64 sequences x 8 heads
-// (fp16): 3.4 us; 4 int8 prompts of 1500-2500 tokens x 8 heads: 7.1 us for 9 MB. The
+// (fp16): 3.4 us; 4 int8 prompts of 1500-2500 tokens x 8 heads: 7.6 us for 9 MB. The
 // loads of a tile are all in flight at once.
 // =============================================================================
 // Exchanges x's lanes with bit M set and y's without: afterwards a lane without it
@@ -271,10 +272,11 @@ DEV void index_read(const IndexReadParams& P) {
 }
 
 // =============================================================================
-// Selection. The bound of q . k over a page is sum_d max(q_d lo_d, q_d hi_d) =
-// [min(q, 0), max(q, 0)] . [lo, hi], a product over 2 T dims; q and the bounds are
-// int8 codes, so the sum is exact on v_mfma_i32_16x16x64_i8 (at most 128 x 127 x
-// 127 < 2^24: exact in fp32 too) and the score
+// Selection. Over a page q . k is at most sum_d max(q_d lo_d, q_d hi_d) =
+// [min(q, 0), max(q, 0)] . [lo, hi], a product over 2 T dims. Here q and the bounds are
+// int8 codes, each the nearest: an estimate of that sum, not a bound. The codes' own sum
+// is exact on v_mfma_i32_16x16x64_i8 (at most 128 x 127 x 127 < 2^24: exact in fp32 too),
+// and the score
 //     max over the group's heads of fp32(fp32(dot * page scale) * head scale)
 // has the same bits however it is computed. Scores are kept as ordered 32-bit keys
 // (larger key = chosen earlier). The pages that are always kept are not scored.
@@ -285,9 +287,9 @@ DEV void index_read(const IndexReadParams& P) {
 // (vk_page_topk).
 //
 // Bound: the rate at which rows of 2 T codes at unrelated addresses arrive. 64 sequences
-// of 512 pages x 8 heads (T = 128): 17.4 us, 69 MB at 4.0 TB/s, where a kernel of these
-// loads alone takes 12.5; 32 of 2048: 34.6 us, 136 MB, the loads alone 27. One sequence of
-// 375 pages: 7.4 us, of which an empty launch is 4.7.
+// of 512 pages x 8 heads (T = 128), 69 MB: 15.8 us where the last-level cache holds the
+// codes (as calls on one layer leave them), 19.3 from HBM, 3.6 TB/s; 32 of 2048, 136 MB: 27.7
+// and 35. One sequence of 375 pages: 6.7 and 7.5 us, of which an empty launch is 4.7.
 // =============================================================================
 
 // What a workgroup of the selection knows of its (sequence, KV head).
@@ -352,10 +354,12 @@ DEV void query_codes(const SelectParams& P, int unit, float (&x)[T / WAVE], int8
 // A wave's turn of 64 scored pages: their ids, codes and scales. keys[i] is page u.lo + i.
 // Codes are loaded in the operands' order, or BY_ROW, a row by adjacent lanes (LPR each),
 // and change lanes in LDS. A CU takes 36 GB/s in the operands' order, where adjacent lanes
-// read 16 rows, and 95 by rows, so few (sequence, KV head)s load by rows (one sequence of
-// 375 pages x 8 heads: 7.5 us against 8.5, 8 of 512: 8.9 against 10.2); all CUs together
-// reach HBM's rate either way, and the operands' order takes fewer registers and no LDS
-// (64 sequences of 512 pages: 18.4 us against 19.6, 32 of 2048: 36.7 against 40).
+// read 16 rows, and 95 by rows, so fewer (sequence, KV head)s than CUs load by rows (one
+// sequence of 375 pages x 8 heads: 6.7 us against 7.3 in the operands' order, 8 of 512: 7.2
+// against 8.5, 31 of 512: 8.9 either way); the operands' order takes fewer registers and no
+// LDS, so that more workgroups share a CU (64 sequences of 512 pages: 15.8 us against 20.3 by
+// rows; 32 of 2048, a workgroup a CU, 27.7 against 26.5). The keys of long contexts of few
+// (vk_page_scores) are loaded in the operands' order too; by rows is not built there.
 template <int T, bool BY_ROW>
 struct PageTurn {
   static constexpr int KJ = 2 * T / 64;                                         // products of 64 dims
@@ -606,7 +610,7 @@ DEV void page_select(const SelectParams& P) {
   __shared__ uint32_t keys[kSelPages];
   __shared__ SelScratch scratch;
   // each XCD takes a run of the units, so that the heads of a sequence, whose rows lie side by
-  // side, are read through one cache (64 sequences of 512 pages: 18.4 -> 17.5 us)
+  // side, are read through one cache (64 sequences of 512 pages: 0.9 us less)
   const int units = P.n_seqs * P.n_kv_heads, run = units / 8, b = (int)blockIdx.x;
   const int unit = b < 8 * run ? (b & 7) * run + (b >> 3) : b;
   float x[T / WAVE];
@@ -665,10 +669,11 @@ DEV void page_topk(const SelectParams& P) {
 // p enters it as two fp16 parts, p = hi + lo to 2^-22 relative (fp32 pools: fp32
 // throughout); the maximum is that of p times the value's scale, so that what is
 // rounded to fp16 lies in (0, 2^15].
-// Bound: HBM where the (sequence, KV head)s fill the CUs. 64 sequences of 64 listed
-// pages x 8 heads, fp16: 45.4 us, 270 MB at 6.0 TB/s; 32 of 128 pages, int8: 29 us, 4.6
-// TB/s with the launch and the chain of list, table and first tile. Few sequences: that
-// chain, then the merge (one sequence of 64 pages: 7.2 + 3.0 us).
+// Bound: HBM where the (sequence, KV head)s fill the CUs. 64 sequences of 64 listed pages x
+// 8 heads, a call from HBM: fp16 47.8 us, 270 MB at 5.7 TB/s; fp32 92.4 us, 5.8 TB/s; int8 of
+// a scale per token 29.8 us, 4.7 TB/s, and per tile 29.2 us, 4.7 TB/s, with the launch and the
+// chain of list, table and first tile. Few sequences: that chain, then the merge (one
+// sequence of 64 pages: 7.1 + 3.3 us).
 // =============================================================================
 constexpr float kShift = 11.0f;           // p is held times 2^11: fp16 subnormals begin 2^-36 below the largest
 constexpr float kRaise = 4.0f;            // the maximum is raised when a score passes it by 2^4
@@ -1028,7 +1033,7 @@ DEV void sparse_attn(const SparseParams& P) {
 }
 
 // Joins the parts of a row: one wave a row, T / 64 dims a lane; lane v holds part v's
-// maximum and sum, 64 parts a turn. Bound: launch and one round of loads, 2.2-4 us.
+// maximum and sum, 64 parts a turn. Bound: launch and one round of loads, 2.3-4.5 us.
 template <int T>
 DEV void sparse_merge(const SparseParams& P) {
   constexpr int EPL = T / WAVE, UN = 8;

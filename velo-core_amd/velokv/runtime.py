@@ -268,7 +268,7 @@ class Context:
                      n_seqs: int, n_heads: int, max_context_len: int, n_first: int = 1, n_last: int = 1,
                      block_tables=None, bt_stride: int = 0, seq_rows=None, workspace=None, workspace_bytes: int = 0,
                      stream=None):
-        """vk_select_pages: the n_pages best pages of each (sequence, KV head) by their bounds, ascending, into
+        """vk_select_pages: the n_pages best pages of each (sequence, KV head) by their bounds' codes, ascending, into
         pages (int32 [n_seqs][n_kv_heads][n_pages], -1 after a list's end)."""
         a = _capi.SparseArgs(layer, _addr(q), q_dtype, None, _addr(pages), n_pages, n_first, n_last,
                              _addr(block_tables), bt_stride, _addr(seq_rows), _addr(context_lens), n_seqs, n_heads,
